@@ -40,7 +40,9 @@ typedef enum {
 typedef enum {
   SRSWA_F32 = 0, SRSWA_BF16 = 1, SRSWA_F16 = 2,
   /* fp8 K/V caches of the paged serving kernels (kv_fp8 fields) */
-  SRSWA_FP8_E4M3FN = 3, SRSWA_FP8_E4M3FNUZ = 4, SRSWA_FP8_E5M2 = 5, SRSWA_FP8_E5M2FNUZ = 6
+  SRSWA_FP8_E4M3FN = 3, SRSWA_FP8_E4M3FNUZ = 4, SRSWA_FP8_E5M2 = 5, SRSWA_FP8_E5M2FNUZ = 6,
+  /* with SRSWA_FP8_E4M3FN, the formats of the scaled 8-bit cache (kv_dtype fields) */
+  SRSWA_I8 = 7
 } srswa_dtype;
 
 /* Library version, e.g. 100 for 0.1.0. */
@@ -980,6 +982,118 @@ typedef struct {
 /* workspace: the per-(row, block) gradient weights, B * nblk * S fp32 */
 int srswa_bm_score_bwd_workspace(const srswa_bm_score_bwd_args* a, size_t* scratch_bytes);
 int srswa_bm_score_bwd(const srswa_bm_score_bwd_args* a, void* scratch, size_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The scaled 8-bit paged cache (no counterpart in the reference).  K and V
+ * pages [num_pages, page_size, HKV, D] hold int8 or float8_e4m3fn values with
+ * one fp32 scale per (page, kv head), a stored value standing for byte * scale.
+ * D 64 or 128, page_size a multiple of 16 up to 1024, rows 16-byte aligned.
+ * A page id outside [0, num_pages) is no page: it is never read or written and
+ * its keys are not visible.
+ *
+ * Append: request r's new tokens, rows cu_seqlens[r] .. cu_seqlens[r + 1) of k /
+ * v, become its keys start[r], start[r] + 1, ...  For each page they touch and
+ * each head, need = 2^e, the smallest power of two (e >= -100) with
+ * max |x| <= QMAX 2^e over the page's new finite values (QMAX 448 / 127); the
+ * scale becomes need where the page's first key is new, else max(scale, need),
+ * and older keys of the page are rounded again when it grew.  Round to nearest
+ * even; infinities saturate; NaN stays NaN in e4m3 and is 0 in int8.  Rows
+ * behind the last new token are left as they are.  Two requests of one call
+ * must not write the same page.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  const void* k;        int64_t k_sn, k_sh;            /* [total, HKV, D] bf16 / fp16       */
+  const void* v;        int64_t v_sn, v_sh;
+  void* k_cache;        int64_t kc_sp, kc_st, kc_sh;   /* [num_pages, page_size, HKV, D]    */
+  void* v_cache;        int64_t vc_sp, vc_st, vc_sh;
+  float* k_scale;       int64_t ks_sp, ks_sh;          /* [num_pages, HKV]                  */
+  float* v_scale;       int64_t vs_sp, vs_sh;
+  const int32_t* block_table; int64_t bt_sr;           /* [R, max_blocks] page ids          */
+  const int32_t* start;                                /* [R] keys already stored           */
+  const int32_t* cu_seqlens;                           /* [R + 1]; NULL: max_new_len rows each */
+  int32_t R, total, max_new_len, HKV, D, max_blocks, num_pages, page_size;
+  int32_t dtype, kv_dtype;
+} srswa_cache8_append_args;
+
+int srswa_cache8_append(const srswa_cache8_append_args* a, void* stream);
+
+/* Attention over that cache.  Request r holds seq_lens[r] keys, the last of
+ * them its query rows' own: row t of qlen sits at p = seq_lens[r] - qlen + t.
+ *   topk NULL: key j is visible when j <= p and (window == 0, or j > p - window,
+ *              or j < sinks);  logit = scale * q.k
+ *   topk:      (decode only) the window keys j > p - window without a bias, and
+ *              the keys before the window of the listed blocks (page_size keys
+ *              each, -1 = empty, a repeated id counts once) with the slot's bias.
+ * A row without a visible key gives 0 (lse -inf).  Rows of q beyond the
+ * requests' are left as they are.  P and V are multiplied in bf16 (V's bytes are
+ * exact there), q and K in q's type; sums and statistics are fp32.
+ * srswa_cache8_decode: a few rows per request (max_query_len each when
+ * cu_seqlens_q is NULL), split over the keys; srswa_cache8_prefill: many. */
+typedef struct {
+  const void* q;        int64_t q_sn, q_sh;            /* [total_q, HQ, D] bf16 / fp16      */
+  const void* k_cache;  int64_t k_sp, k_st, k_sh;
+  const void* v_cache;  int64_t v_sp, v_st, v_sh;
+  const float* k_scale; int64_t ks_sp, ks_sh;
+  const float* v_scale; int64_t vs_sp, vs_sh;
+  const int32_t* block_table; int64_t bt_sr;           /* [R, max_blocks]                   */
+  const int32_t* seq_lens;                             /* [R]                               */
+  const int32_t* cu_seqlens_q;                         /* [R + 1] or NULL                   */
+  const int32_t* topk;  int64_t t_sh, t_sn, t_sk;      /* [HKV, total_q, topk_n] or NULL    */
+  const float* bias;                                   /* same strides as topk; NULL = 0    */
+  void* out;            int64_t o_sn, o_sh;            /* [total_q, HQ, D]                  */
+  float* lse;           int64_t lse_sn, lse_sh;        /* [total_q, HQ] natural log or NULL */
+  int32_t R, total_q, max_query_len, HQ, HKV, D, topk_n, max_blocks, num_pages, page_size;
+  int32_t window, sinks;
+  float scale;
+  int32_t dtype, kv_dtype;
+} srswa_cache8_attend_args;
+
+size_t srswa_cache8_decode_workspace(const srswa_cache8_attend_args* a);
+int srswa_cache8_decode(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream);
+size_t srswa_cache8_prefill_workspace(const srswa_cache8_attend_args* a);
+int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Pages of a pool: dealing, reordering (sharing, copying, freeing), compacting.
+ * State: block_table [R, W] page ids (-1 = none), seq_lens [R], ref [num_pages]
+ * (how many rows hold a page; 0 = free).  Every call reads one state and writes
+ * another (the outputs must not overlap the inputs); page data moves in place,
+ * in every cache listed: page i of a cache is the `bytes` bytes at base + i *
+ * stride (bytes too).  Free pages are taken lowest first, so results do not
+ * depend on the order of execution.
+ *   reserve: row r gets pages for keys [0, lens[r]) where it has none, in row
+ *            and block order; seq_lens_out = lens; count = pages missing (their
+ *            entries stay -1).
+ *   reorder: row r continues row parents[r] (outside [0, R): it becomes empty).
+ *            Pages before the last, begun one are shared; the first child of a
+ *            parent keeps its other pages, any later child gets a copy of the
+ *            begun page; rows that nobody continues give up theirs; count =
+ *            copies that found no free page (their entries stay -1).
+ *   compact: with n pages held, the held pages at or past n move, in order, to
+ *            the free ones below n, and the table follows; count = n.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  void* base;
+  int64_t stride, bytes;
+} srswa_page_cache;
+
+typedef struct {
+  const int32_t* block_table;  int64_t bt_sr;          /* [R, W]                            */
+  const int32_t* seq_lens;                             /* [R]                               */
+  const int32_t* ref;                                  /* [num_pages]                       */
+  const int32_t* rows;                                 /* reserve: lens [R]; reorder: parents [R] */
+  int32_t* block_table_out;    int64_t bto_sr;
+  int32_t* seq_lens_out;
+  int32_t* ref_out;
+  int32_t* count;                                      /* [1]                               */
+  const srswa_page_cache* caches;                      /* host array of ncaches             */
+  int32_t ncaches, R, W, num_pages, page_size;
+} srswa_pages_args;
+
+size_t srswa_pages_workspace(const srswa_pages_args* a);
+int srswa_pages_reserve(const srswa_pages_args* a, void* ws, size_t ws_bytes, void* stream);
+int srswa_pages_reorder(const srswa_pages_args* a, void* ws, size_t ws_bytes, void* stream);
+int srswa_pages_compact(const srswa_pages_args* a, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

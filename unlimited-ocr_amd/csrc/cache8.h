@@ -1,0 +1,76 @@
+// Shared pieces of the scaled 8-bit paged cache (float8_e4m3fn or int8 values,
+// one fp32 scale per page and kv head): conversions and the page geometry.
+#pragma once
+
+#include "common.h"
+
+namespace srswa {
+
+constexpr int kI8 = SRSWA_I8;
+constexpr int kScaleMinExp = -100;   // a page of zeros has scale 2^-100
+
+template <int KV> constexpr float kQMax = KV == kI8 ? 127.f : 448.f;
+
+// The smallest power of two s >= 2^kScaleMinExp with a <= QMAX s, for finite
+// a >= 0.  With a = 1.m 2^x (fp32 fields) and QMAX = 1.f 2^w the exponent is
+// x - w, one more when m > f: no division and no rounding.  (A subnormal a has
+// x = -127 and falls to the minimum.)
+template <int KV>
+__device__ __forceinline__ float scale_for(float a) {
+  constexpr int w = KV == kI8 ? 6 : 8;                          // 127 = 1.984375 2^6, 448 = 1.75 2^8
+  constexpr uint32_t f = KV == kI8 ? 0x7e0000u : 0x600000u;
+  const uint32_t u = __float_as_uint(a);
+  const int e = max((int)(u >> 23) - 127 - w + ((u & 0x7fffffu) > f ? 1 : 0), kScaleMinExp);
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// four values in units of the scale -> four bytes, round to nearest even,
+// saturating; NaN stays NaN in e4m3 and becomes 0 in int8
+template <int KV>
+__device__ __forceinline__ uint32_t to_bytes4(const float* y) {
+  if constexpr (KV == kI8) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float c = y[i] == y[i] ? fminf(fmaxf(rintf(y[i]), -127.f), 127.f) : 0.f;
+      w |= ((uint32_t)(int)c & 0xffu) << (8 * i);
+    }
+    return w;
+  } else {
+    float c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = y[i] == y[i] ? fminf(fmaxf(y[i], -448.f), 448.f) : y[i];
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], w, true);
+    return (uint32_t)w;
+  }
+}
+
+__device__ __forceinline__ float i8_f32(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+
+// four bytes -> fp32, in units of the scale
+template <int KV>
+__device__ __forceinline__ void from_bytes4(uint32_t w, float* f) {
+  if constexpr (KV == kI8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i8_f32(w, i);
+  } else {
+    const f32x2_t a = fp8x2_f32<KV, false>(w), b = fp8x2_f32<KV, true>(w);
+    f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
+  }
+}
+
+// four bytes -> four values of T, two words (exact: every e4m3 and int8 value
+// is a bf16 and an fp16 value)
+template <int KV, typename T>
+__device__ __forceinline__ uint2 bytes4_to(uint32_t w) {
+  if constexpr (KV == kI8) {
+    const float a = i8_f32(w, 0), b = i8_f32(w, 1), c = i8_f32(w, 2), d = i8_f32(w, 3);
+    if constexpr (std::is_same<T, bf16_t>::value) return make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+    else return make_uint2(pack_h16x2(a, b), pack_h16x2(c, d));
+  } else {
+    return make_uint2(fp8x2_to<KV, T, false>(w), fp8x2_to<KV, T, true>(w));
+  }
+}
+
+}  // namespace srswa

@@ -1,0 +1,593 @@
+// Attention of a few query rows per request over the scaled 8-bit paged cache
+// (gfx950): every key, a sliding window with first tokens that stay visible, or
+// selected blocks.
+//
+// One workgroup = (request, kv head, 16-row tile, chunk of keys); its rows are
+// the tile's (token, query head of the group) pairs, so a K/V byte is loaded
+// once for all of them.  Four waves take units of 32 keys in turn, entirely in
+// registers:
+//   S^T = K Q^T   v_mfma_f32_16x16x32: A = 16 keys x 32 dims.  The reduction
+//         runs over the dims in any order, so a lane takes 16 contiguous bytes
+//         of a key row per load (two steps) and Q's operand follows suit.
+//   D layout: lane l holds row l % 16 and keys 4 (l / 16) + 0..3 of each of the
+//         unit's two 16-key groups, which is an A operand of P with its keys in
+//         a fixed order (slot j < 4: group 0, j >= 4: group 1);
+//   O += P V  v_mfma_f32_16x16x32_bf16: a lane loads D / 16 contiguous bytes of
+//         each of its 8 keys (the 16 lanes of a key cover its row), and an 8 x 8
+//         byte transpose by v_perm_b32 gives it the 8 keys of one dim per MFMA.
+// A 16-key group lies in one page (page sizes are multiples of 16), so the K
+// scale joins the softmax scale and the V scale multiplies P, in fp32, before P
+// is rounded to bf16 (2^-9 of each weight; the sum l adds the unrounded ones).
+// The running maximum moves only when a logit exceeds it by 2^8.
+// Chunks of one tile are joined by cache8_merge_kernel.
+#include <algorithm>
+
+#include "cache8.h"
+#include "mfma_common.h"
+
+namespace srswa {
+namespace {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kRows = 16;
+constexpr int kGroup = 16;     // keys per page lookup; a unit is two groups
+
+struct AttendK {
+  srswa_cache8_attend_args a;
+  int G;                  // query heads per kv head
+  int tiles, nchunk, upc; // row tiles and chunks per (request, kv head), units per chunk
+  int rs;                 // rows of a record
+  int gpp;                // 16-key groups per page
+  float scale_l2;         // scale * log2(e)
+  float* part;            // records: [R * tiles * HKV][nchunk][rs * (D + 2)]
+};
+
+// What a row tile reads, the same on every thread and in the merge kernel.
+struct Tile {
+  int row0, nrows;        // rows of the tile: (token t, head g) = (row / G, row % G)
+  int q0;                 // first query token of the request
+  int p0;                 // position of the request's first query row
+  int pmin, pmax;         // positions of the tile's first and last row
+  int kend;               // keys that have a table entry
+  int ng0, g1, units;     // groups of the first section, first group of the second, units in all
+};
+
+template <bool SEL>
+__device__ __forceinline__ Tile tile_of(const AttendK& p, int r, int tile) {
+  const srswa_cache8_attend_args& a = p.a;
+  Tile t;
+  const int q0 = a.cu_seqlens_q ? min(max(a.cu_seqlens_q[r], 0), a.total_q) : r * a.max_query_len;
+  const int q1 = a.cu_seqlens_q ? min(max(a.cu_seqlens_q[r + 1], q0), a.total_q) : q0 + a.max_query_len;
+  const int sl = max(a.seq_lens[r], 0);
+  t.q0 = q0;
+  t.p0 = sl - (q1 - q0);
+  if constexpr (SEL) {                        // the heads of one token, 16 at a time
+    const int per = (p.G + kRows - 1) / kRows;
+    const int tok = tile / per, g0 = tile % per * kRows;
+    t.row0 = tok * p.G + g0;
+    t.nrows = tok < q1 - q0 ? min(kRows, p.G - g0) : 0;
+  } else {
+    t.row0 = tile * kRows;
+    t.nrows = (int)max((int64_t)0, min((int64_t)kRows, (int64_t)(q1 - q0) * p.G - t.row0));
+  }
+  t.kend = (int)min((int64_t)sl, (int64_t)a.max_blocks * a.page_size);
+  t.pmin = t.p0 + t.row0 / p.G;
+  t.pmax = t.nrows > 0 ? t.p0 + (t.row0 + t.nrows - 1) / p.G : -1;
+  const int end = min(t.pmax + 1, t.kend);    // keys some row may see: [0, end)
+  const int lo = a.window > 0 ? max(t.pmin - a.window + 1, 0) : 0;
+  if constexpr (SEL) {
+    t.ng0 = a.topk_n * p.gpp;                 // each slot's block, group by group
+    t.g1 = lo / kGroup;
+  } else {
+    t.ng0 = lo > 0 ? (min(min(a.sinks, lo), max(end, 0)) + kGroup - 1) / kGroup : 0;   // first tokens
+    t.g1 = max(lo / kGroup, t.ng0);
+  }
+  const int ng1 = SEL && a.window == 0 ? 0 : max((end + kGroup - 1) / kGroup - t.g1, 0);
+  t.units = t.nrows > 0 ? (t.ng0 + ng1 + 1) / 2 : 0;
+  return t;
+}
+
+// 4 x 4 byte transpose: word t of the result holds byte t of a, b, c, d
+__device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t* o) {
+  const uint32_t ab0 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab1 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+  const uint32_t cd0 = __builtin_amdgcn_perm(d, c, 0x05010400u), cd1 = __builtin_amdgcn_perm(d, c, 0x07030602u);
+  o[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u);
+  o[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
+  o[2] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u);
+  o[3] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4_t mfma16(const uint4& a, const uint4& b, f32x4_t c) {
+  if constexpr (std::is_same<T, bf16_t>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+}
+
+__device__ __forceinline__ float xor16_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor16_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// One unit's K and V bytes of a lane.
+template <int D>
+struct UnitBytes {
+  static constexpr int DV = D / 16;                    // bytes per V key and lane
+  uint4 k[2][D / 64];                                  // key l % 16 of each group
+  std::conditional_t<DV == 8, uint2, uint32_t> v[8];   // keys 4 (l / 16) + 0..3 of each group
+};
+
+template <typename T, int KV, int D, bool SEL>
+__global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
+  constexpr int NL = D / 64;      // K loads per group
+  constexpr int DV = D / 16;      // V tiles
+  using VB = std::conditional_t<DV == 8, uint2, uint32_t>;
+  __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
+  __shared__ __align__(16) float s_o[kWaves][kRows][D];
+  const srswa_cache8_attend_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int n = lane & 15, g = lane >> 4;
+
+  // the heads of one chunk run side by side (their rows share DRAM pages); a
+  // tile's later chunks come after every tile's earlier ones
+  int lid = (int)blockIdx.x;
+  const int h = lid % a.HKV;
+  lid /= a.HKV;
+  const int rt = lid % (a.R * p.tiles), chunk = lid / (a.R * p.tiles);
+  const int r = rt / p.tiles;
+  const Tile t = tile_of<SEL>(p, r, rt % p.tiles);
+  if (t.nrows == 0 || (chunk > 0 && chunk * p.upc >= t.units)) return;
+  const int u_end = min(t.units, (chunk + 1) * p.upc);
+
+  // Q operand: lane (row n, g) holds dims 64 i + 16 g + 8 e .. + 7 of step 2 i + e
+  const int row = min(t.row0 + n, t.row0 + t.nrows - 1);
+  const int tok = row / p.G, hq = h * p.G + row % p.G;
+  uint4 qf[2 * NL];
+  {
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(t.q0 + tok) * a.q_sn + (int64_t)hq * a.q_sh + 16 * g;
+#pragma unroll
+    for (int s = 0; s < 2 * NL; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + 64 * (s / 2) + 8 * (s % 2));
+  }
+  const int pr = n < t.nrows ? t.p0 + tok : -1;        // this lane's row position
+  const int end = min(t.pmax + 1, t.kend);
+  const int wlo = a.window > 0 ? t.pmin - a.window : INT_MIN;   // every row's window starts past wlo
+  const int32_t* topk = nullptr;
+  const float* bias = nullptr;
+  if constexpr (SEL) {
+    const int64_t o = (int64_t)h * a.t_sh + (int64_t)(t.q0 + t.row0 / p.G) * a.t_sn;
+    topk = a.topk + o;
+    bias = a.bias ? a.bias + o : nullptr;
+  }
+
+  f32x4_t acc[DV];
+#pragma unroll
+  for (int d = 0; d < DV; ++d) acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, msub = 0.f, thr = -INFINITY, l = 0.f;
+
+  const uint8_t* kcache = reinterpret_cast<const uint8_t*>(a.k_cache) + (int64_t)h * a.k_sh;
+  const uint8_t* vcache = reinterpret_cast<const uint8_t*>(a.v_cache) + (int64_t)h * a.v_sh;
+  const int64_t koff = (int64_t)n * a.k_st + 16 * g;
+  const int64_t voff = (int64_t)(4 * g) * a.v_st + DV * n;
+
+  for (int u0 = chunk * p.upc + wave; u0 < u_end; u0 += kWaves * kWave) {
+    // lane i looks up the two groups of this wave's i-th unit from here: first
+    // key (-1: nothing to see), page and row in it, scales, bias and bounds
+    int dk[2], dpage[2], drow[2], dlo[2], dhi[2];
+    float dks[2], dvs[2], db[2];
+    bool whole = true;
+    const int du = u0 + kWaves * lane;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int gi = 2 * du + e;
+      int key = -1;
+      db[e] = 0.f;
+      dlo[e] = 0;
+      dhi[e] = INT_MAX;
+      if (du < u_end) {
+        if (gi < t.ng0) {
+          if constexpr (SEL) {
+            const int slot = gi / p.gpp, sub = gi % p.gpp;
+            const int id = topk[(int64_t)slot * a.t_sk];
+            bool ok = id >= 0 && id < a.max_blocks;
+            for (int s = 0; s < slot; ++s) ok = ok && topk[(int64_t)s * a.t_sk] != id;
+            if (ok) key = id * a.page_size + sub * kGroup;
+            dhi[e] = t.pmin - a.window;                // remote keys end before the window
+            if (bias) {                                  // the lowest finite value stays finite in log2 units
+              const float b = bias[(int64_t)slot * a.t_sk];
+              db[e] = b > -INFINITY && b * kLog2e < -3.0e38f ? -3.0e38f : b * kLog2e;
+            }
+          } else {
+            key = gi * kGroup;
+          }
+        } else {
+          key = (t.g1 + gi - t.ng0) * kGroup;
+          if constexpr (SEL) dlo[e] = t.pmin - a.window + 1;
+        }
+        if (key >= end || (SEL && key > dhi[e])) key = -1;
+      }
+      int page = -1;
+      if (key >= 0) page = a.block_table[(int64_t)r * a.bt_sr + key / a.page_size];
+      const bool ok = page >= 0 && page < a.num_pages;
+      dk[e] = ok ? key : -1;
+      dpage[e] = ok ? page : 0;
+      drow[e] = ok ? key % a.page_size : 0;
+      dks[e] = ok ? p.scale_l2 * a.k_scale[(int64_t)page * a.ks_sp + (int64_t)h * a.ks_sh] : 0.f;
+      dvs[e] = ok ? a.v_scale[(int64_t)page * a.vs_sp + (int64_t)h * a.vs_sh] : 0.f;
+      const int last = key + kGroup - 1;
+      if constexpr (SEL)
+        whole = whole && ok && key >= dlo[e] && last <= dhi[e] && last < end;
+      else
+        whole = whole && ok && last <= t.pmin && last < t.kend &&
+                (a.window == 0 || key > t.pmax - a.window || last < a.sinks);
+    }
+    const uint64_t whole_bits = __ballot(whole);
+    const int cnt = min(kWave, (u_end - u0 + kWaves - 1) / kWaves);
+
+    auto load = [&](int i, UnitBytes<D>& b) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int page = __builtin_amdgcn_readlane(dpage[e], i), rw = __builtin_amdgcn_readlane(drow[e], i);
+        const uint8_t* kp = kcache + (int64_t)page * a.k_sp + (int64_t)rw * a.k_st + koff;
+        const uint8_t* vp = vcache + (int64_t)page * a.v_sp + (int64_t)rw * a.v_st + voff;
+#pragma unroll
+        for (int q = 0; q < NL; ++q) b.k[e][q] = *reinterpret_cast<const uint4*>(kp + 64 * q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b.v[4 * e + j] = *reinterpret_cast<const VB*>(vp + (int64_t)j * a.v_st);
+      }
+    };
+    UnitBytes<D> nx;
+    load(0, nx);
+    for (int i = 0; i < cnt; ++i) {
+      UnitBytes<D> b = nx;
+      if (i + 1 < cnt) load(i + 1, nx);
+      // S^T
+      f32x4_t sc[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sc[e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < NL; ++q) {
+          const uint2 k0 = bytes4_to<KV, T>(b.k[e][q].x), k1 = bytes4_to<KV, T>(b.k[e][q].y);
+          const uint2 k2 = bytes4_to<KV, T>(b.k[e][q].z), k3 = bytes4_to<KV, T>(b.k[e][q].w);
+          sc[e] = mfma16<T>(make_uint4(k0.x, k0.y, k1.x, k1.y), qf[2 * q], sc[e]);
+          sc[e] = mfma16<T>(make_uint4(k2.x, k2.y, k3.x, k3.y), qf[2 * q + 1], sc[e]);
+        }
+      }
+      float z[8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dks[e]), i));
+        const float bl = SEL ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(db[e]), i)) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[4 * e + j] = SEL ? fmaf(sc[e][j], ks, bl) : sc[e][j] * ks;
+      }
+      if (!((whole_bits >> i) & 1)) {
+        // some key is not visible to some row: its logit is -inf, and a key no
+        // row sees has its V bytes cleared (0 * NaN would reach O)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = __builtin_amdgcn_readlane(dk[e], i) ;
+          const int lo = SEL ? __builtin_amdgcn_readlane(dlo[e], i) : 0;
+          const int hi = SEL ? __builtin_amdgcn_readlane(dhi[e], i) : 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int k = key + 4 * g + j;
+            bool see = key >= 0 && k <= pr && k < t.kend, any = key >= 0 && k < end;
+            if constexpr (SEL) {
+              see = see && k >= lo && k <= hi;
+              any = any && k >= lo && k <= hi;
+            } else if (a.window > 0) {
+              see = see && (k > pr - a.window || k < a.sinks);
+              any = any && (k > wlo || k < a.sinks);
+            }
+            z[4 * e + j] = see ? z[4 * e + j] : -INFINITY;
+            if constexpr (DV == 8) {
+              b.v[4 * e + j].x = any ? b.v[4 * e + j].x : 0u;
+              b.v[4 * e + j].y = any ? b.v[4 * e + j].y : 0u;
+            } else {
+              b.v[4 * e + j] = any ? b.v[4 * e + j] : 0u;
+            }
+          }
+        }
+      }
+      float zm = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+      if (__any(zm > thr)) {
+        zm = xor32_max(xor16_max(zm));
+        const float mn = fmaxf(m, zm);
+        const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
+        m = mn;
+        msub = mn == -INFINITY ? 0.f : mn;
+        thr = mn + 8.f;
+        l *= alpha;
+        float ar[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ar[j] = __shfl(alpha, 4 * g + j, kWave);
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[d][j] *= ar[j];
+      }
+      const float vs0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dvs[0]), i));
+      const float vs1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dvs[1]), i));
+      float pe[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        pe[j] = __builtin_amdgcn_exp2f(z[j] - msub);
+        l += pe[j];
+        pe[j] *= j < 4 ? vs0 : vs1;
+      }
+      const uint4 pa = make_uint4(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3]), pack_bf16x2(pe[4], pe[5]),
+                                  pack_bf16x2(pe[6], pe[7]));
+      // O += P V
+#pragma unroll
+      for (int hf = 0; hf < DV / 4; ++hf) {
+        uint32_t w[8], ta[4], tb[4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (DV == 8) w[j] = hf ? b.v[j].y : b.v[j].x;
+          else w[j] = b.v[j];
+        }
+        transpose4(w[0], w[1], w[2], w[3], ta);
+        transpose4(w[4], w[5], w[6], w[7], tb);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const uint2 x0 = bytes4_to<KV, bf16_t>(ta[d]), x1 = bytes4_to<KV, bf16_t>(tb[d]);
+          acc[4 * hf + d] = mfma16<bf16_t>(pa, make_uint4(x0.x, x0.y, x1.x, x1.y), acc[4 * hf + d]);
+        }
+      }
+    }
+  }
+
+  // the four waves' (m, l, O) of the tile: O lane layout row 4 g + j, dims DV n + d
+  l = xor32_sum(xor16_sum(l));
+  if (g == 0) {
+    s_m[wave][n] = m;
+    s_l[wave][n] = l;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (4 * g + j < t.nrows) {
+#pragma unroll
+      for (int d = 0; d < DV; d += 4)
+        *reinterpret_cast<float4*>(&s_o[wave][4 * g + j][DV * n + d]) =
+            make_float4(acc[d][j], acc[d + 1][j], acc[d + 2][j], acc[d + 3][j]);
+    }
+  __syncthreads();
+  const bool only = t.units <= p.upc;
+  float* rec = only ? nullptr : p.part + ((int64_t)(rt * a.HKV + h) * p.nchunk + chunk) * p.rs * (D + 2);
+  for (int i = tid; i < t.nrows * (D / 4); i += kThreads) {
+    const int rr = i / (D / 4), c = i % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][rr]);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = s_m[w][rr] == -INFINITY ? 0.f : exp2f(s_m[w][rr] - M);
+      const float4 x = *reinterpret_cast<const float4*>(&s_o[w][rr][c]);
+      L = fmaf(f, s_l[w][rr], L);
+      o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+    }
+    if (only) {
+      const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
+      const float inv = M == -INFINITY ? 0.f : 1.f / L;
+      T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn + (int64_t)ho * a.o_sh + c;
+      uint2 w;
+      w.x = Mfma<T>::pack2(o.x * inv, o.y * inv);
+      w.y = Mfma<T>::pack2(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(op) = w;
+      if (a.lse && c == 0)
+        a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] =
+            M == -INFINITY ? -INFINITY : (M + log2f(L)) * kLn2;
+    } else {
+      *reinterpret_cast<float4*>(rec + rr * D + c) = o;
+      if (c == 0) {
+        rec[p.rs * D + rr] = M;
+        rec[p.rs * D + p.rs + rr] = L;
+      }
+    }
+  }
+}
+
+// Joins a tile's chunks: one workgroup per (request, tile, kv head).
+template <typename T, int D, bool SEL>
+__global__ __launch_bounds__(kThreads) void cache8_merge_kernel(AttendK p) {
+  const srswa_cache8_attend_args& a = p.a;
+  const int h = (int)blockIdx.x % a.HKV, rt = (int)blockIdx.x / a.HKV;
+  const Tile t = tile_of<SEL>(p, rt / p.tiles, rt % p.tiles);
+  if (t.nrows == 0 || t.units <= p.upc) return;
+  const int nc = (t.units + p.upc - 1) / p.upc;
+  const int64_t rsz = (int64_t)p.rs * (D + 2);
+  const float* rec = p.part + (int64_t)(rt * a.HKV + h) * p.nchunk * rsz;
+  for (int i = threadIdx.x; i < t.nrows * (D / 4); i += kThreads) {
+    const int rr = i / (D / 4), c = i % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+    for (int k = 0; k < nc; ++k) M = fmaxf(M, rec[k * rsz + p.rs * D + rr]);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < nc; ++k) {
+      const float mk = rec[k * rsz + p.rs * D + rr];
+      const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
+      const float4 x = *reinterpret_cast<const float4*>(rec + k * rsz + rr * D + c);
+      L = fmaf(f, rec[k * rsz + p.rs * D + p.rs + rr], L);
+      o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+    }
+    const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
+    const float inv = M == -INFINITY ? 0.f : 1.f / L;
+    uint2 w;
+    w.x = Mfma<T>::pack2(o.x * inv, o.y * inv);
+    w.y = Mfma<T>::pack2(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn +
+                              (int64_t)ho * a.o_sh + c) = w;
+    if (a.lse && c == 0)
+      a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] =
+          M == -INFINITY ? -INFINITY : (M + log2f(L)) * kLn2;
+  }
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check(const srswa_cache8_attend_args* a, const char* what) {
+  if (!a || !a->q || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale || !a->block_table || !a->seq_lens ||
+      !a->out) {
+    set_error("%s: null argument", what);
+    return SRSWA_INVALID;
+  }
+  if (a->R < 0 || a->total_q < 0 || a->max_query_len < 0 || a->HQ <= 0 || a->HKV <= 0 || a->topk_n < 0 ||
+      a->max_blocks <= 0 || a->num_pages <= 0 || a->page_size <= 0 || a->window < 0 || a->sinks < 0 ||
+      (!a->cu_seqlens_q && (int64_t)a->R * a->max_query_len != a->total_q)) {
+    set_error("%s: bad sizes", what);
+    return SRSWA_INVALID;
+  }
+  if (a->HQ % a->HKV) {
+    set_error("%s: HQ=%d must be a multiple of HKV=%d", what, a->HQ, a->HKV);
+    return SRSWA_UNSUPPORTED;
+  }
+  if (!(a->D == 64 || a->D == 128) || !(a->dtype == SRSWA_BF16 || a->dtype == SRSWA_F16) ||
+      !(a->kv_dtype == SRSWA_I8 || a->kv_dtype == SRSWA_FP8_E4M3FN)) {
+    set_error("%s: D=%d / dtype %d / cache format %d not supported", what, a->D, a->dtype, a->kv_dtype);
+    return SRSWA_UNSUPPORTED;
+  }
+  if (a->page_size % 16 || a->page_size > 1024 || (int64_t)a->max_blocks * a->page_size > (1 << 30) ||
+      a->window > (1 << 30) || a->sinks > (1 << 30)) {
+    set_error("%s: page size %d must be a multiple of 16 up to 1024, and %d of them at most 2^30 keys", what,
+              a->page_size, a->max_blocks);
+    return SRSWA_UNSUPPORTED;
+  }
+  const int64_t qs[] = {a->q_sn, a->q_sh, a->o_sn, a->o_sh};
+  for (int64_t s : qs)
+    if (s % 8) {
+      set_error("%s: strides must keep rows 16-byte aligned", what);
+      return SRSWA_UNSUPPORTED;
+    }
+  const int64_t ks[] = {a->k_sp, a->k_st, a->k_sh, a->v_sp, a->v_st, a->v_sh};
+  for (int64_t s : ks)
+    if (s % 16) {
+      set_error("%s: cache strides must keep rows 16-byte aligned", what);
+      return SRSWA_UNSUPPORTED;
+    }
+  if (!al16(a->q) || !al16(a->k_cache) || !al16(a->v_cache) || !al16(a->out)) {
+    set_error("%s: pointers must be 16-byte aligned", what);
+    return SRSWA_UNSUPPORTED;
+  }
+  if (a->topk && (a->window <= 0 && a->topk_n == 0)) {
+    set_error("%s: selected blocks need slots or a window", what);
+    return SRSWA_INVALID;
+  }
+  return SRSWA_OK;
+}
+
+// Chunks: enough workgroups to fill the GPU several times, at least 16 units
+// (four per wave) and at most 64 each, so that requests of uneven length spread.
+AttendK plan(const srswa_cache8_attend_args* a, bool split) {
+  AttendK p{};
+  p.a = *a;
+  p.G = a->HQ / a->HKV;
+  p.gpp = a->page_size / kGroup;
+  p.scale_l2 = a->scale * kLog2e;
+  const int64_t rows = (int64_t)a->max_query_len * p.G;
+  p.tiles = (int)(a->topk ? (int64_t)a->max_query_len * ((p.G + kRows - 1) / kRows) : (rows + kRows - 1) / kRows);
+  p.rs = (int)std::min<int64_t>(kRows, a->topk ? p.G : rows);
+  const int64_t cap = (int64_t)a->max_blocks * a->page_size;
+  int64_t groups = cap / kGroup;
+  if (a->topk) groups = (int64_t)a->topk_n * p.gpp + std::min<int64_t>(groups, a->window / kGroup + 2);
+  else if (a->window > 0)
+    groups = std::min<int64_t>(groups, ((int64_t)a->window + a->max_query_len) / kGroup + 2 + (a->sinks + kGroup - 1) / kGroup);
+  const int64_t units = (groups + 1) / 2;
+  p.upc = 0x7fffffff / 2;
+  p.nchunk = 1;
+  if (split) {
+    const int64_t w = std::max<int64_t>(1, (int64_t)a->R * a->HKV * p.tiles);
+    p.upc = (int)std::min<int64_t>(64, std::max<int64_t>(16, units * w / 4096));
+    p.nchunk = (int)std::max<int64_t>(1, (units + p.upc - 1) / p.upc);
+  }
+  return p;
+}
+
+size_t ws_bytes_of(const AttendK& p) {
+  return p.nchunk > 1 ? (size_t)p.a.R * p.tiles * p.a.HKV * p.nchunk * p.rs * (p.a.D + 2) * sizeof(float) : 0;
+}
+
+template <typename T, int KV, int D, bool SEL>
+void launch(const AttendK& p, unsigned grid, hipStream_t st) {
+  cache8_decode_kernel<T, KV, D, SEL><<<grid, kThreads, 0, st>>>(p);
+  if (p.nchunk > 1)
+    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.a.R * p.tiles * p.a.HKV), kThreads, 0, st>>>(p);
+}
+template <typename T, int KV, int D>
+void launch_sel(const AttendK& p, unsigned grid, hipStream_t st) {
+  if (p.a.topk) launch<T, KV, D, true>(p, grid, st);
+  else launch<T, KV, D, false>(p, grid, st);
+}
+template <typename T, int KV>
+void launch_d(const AttendK& p, unsigned grid, hipStream_t st) {
+  if (p.a.D == 64) launch_sel<T, KV, 64>(p, grid, st);
+  else launch_sel<T, KV, 128>(p, grid, st);
+}
+template <typename T>
+void launch_kv(const AttendK& p, unsigned grid, hipStream_t st) {
+  if (p.a.kv_dtype == SRSWA_I8) launch_d<T, kI8>(p, grid, st);
+  else launch_d<T, kFp8E4M3FN>(p, grid, st);
+}
+
+int run(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream, bool split, const char* what) {
+  const int rc = check(a, what);
+  if (rc != SRSWA_OK) return rc;
+  if (a->R == 0 || a->total_q == 0 || a->max_query_len == 0) return SRSWA_OK;
+  AttendK p = plan(a, split);
+  const size_t need = ws_bytes_of(p);
+  if (need > 0 && (!ws || ws_bytes < need)) {
+    set_error("%s: workspace of %zu bytes required (got %zu)", what, need, ws_bytes);
+    return SRSWA_WORKSPACE;
+  }
+  p.part = reinterpret_cast<float*>(ws);
+  const int64_t grid = (int64_t)a->R * p.tiles * a->HKV * p.nchunk;
+  if (grid > 0x7fffffff) {
+    set_error("%s: grid too large", what);
+    return SRSWA_UNSUPPORTED;
+  }
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (a->dtype == SRSWA_BF16) launch_kv<bf16_t>(p, (unsigned)grid, st);
+  else launch_kv<__half>(p, (unsigned)grid, st);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) {
+    set_error("%s launch failed: %s", what, hipGetErrorString(e));
+    return SRSWA_LAUNCH;
+  }
+  return SRSWA_OK;
+}
+
+bool plannable(const srswa_cache8_attend_args* a) {
+  return a && a->R > 0 && a->HQ > 0 && a->HKV > 0 && a->page_size >= 16 && a->max_blocks > 0 && a->max_query_len > 0;
+}
+
+}  // namespace
+}  // namespace srswa
+
+using namespace srswa;
+
+extern "C" size_t srswa_cache8_decode_workspace(const srswa_cache8_attend_args* a) {
+  return plannable(a) ? ws_bytes_of(plan(a, true)) : 0;
+}
+extern "C" int srswa_cache8_decode(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream) {
+  return run(a, ws, ws_bytes, stream, true, "cache8 decode");
+}
+extern "C" size_t srswa_cache8_prefill_workspace(const srswa_cache8_attend_args* a) {
+  return plannable(a) ? ws_bytes_of(plan(a, false)) : 0;
+}
+extern "C" int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream) {
+  if (a && a->topk) {
+    set_error("cache8 prefill: selected blocks are for decode");
+    return SRSWA_UNSUPPORTED;
+  }
+  return run(a, ws, ws_bytes, stream, false, "cache8 prefill");
+}

@@ -1,0 +1,503 @@
+// Pages of a pool (gfx950): dealing them out, reordering rows (sharing, copying
+// and freeing pages) and compacting, over block_table [R, W], seq_lens [R] and
+// ref [num_pages] (rows that hold a page, 0 = free).
+//
+// Every step reads the old state and writes the new one, and free pages are
+// found by rank (the k-th free page in ascending order, from counts per tile of
+// kTile pages), so no result depends on the order of execution; the only atomics
+// are integer additions into ref.
+#include <algorithm>
+
+#include "common.h"
+
+namespace srswa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTile = 2048;       // pages per tile of the free-page counts
+constexpr int kMaxCaches = 64;    // caches per copy launch (the table is a kernel argument)
+
+struct PagesK {
+  const int32_t* bt;   int64_t bt_sr;
+  const int32_t* sl;
+  const int32_t* ref;
+  const int32_t* rows;
+  int32_t* bto;        int64_t bto_sr;
+  int32_t* slo;
+  int32_t* refo;
+  int32_t* count;
+  int R, W, N, page_size, ntiles;
+  // workspace
+  int32_t* need;       // [R]       pages a row asks for
+  int32_t* src;        // [R | N]   reorder: the page row r copies; compact: pair i's source
+  int32_t* dst;        // [R | N]   its destination (-1: none)
+  int32_t* tfree;      // [ntiles]  free (compact: held) pages per tile
+  int32_t* npairs;     // [1]
+  uint32_t* bits;      // [ceil(N / 32)] free pages
+};
+
+// sum over the workgroup of one value per thread, on every thread
+__device__ __forceinline__ int block_sum(int v, int* s) {
+  v = wave_sum_int(v);
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = v;
+  __syncthreads();
+  int t = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / kWave; ++w) t += s[w];
+  return t;
+}
+
+// exclusive prefix of one value per thread over the workgroup, and the total
+__device__ __forceinline__ int block_scan(int v, int* s, int* total) {
+  int incl = v;
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int x = __shfl_up(incl, o, kWave);
+    if (lane >= o) incl += x;
+  }
+  __syncthreads();
+  if (lane == kWave - 1) s[w] = incl;
+  __syncthreads();
+  int base = 0, t = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / kWave; ++i) {
+    base += i < w ? s[i] : 0;
+    t += s[i];
+  }
+  *total = t;
+  return base + incl - v;
+}
+
+__device__ __forceinline__ bool valid_page(const PagesK& p, int id) { return id >= 0 && id < p.N; }
+
+// Marks and counts the free pages of one tile of ref.
+__device__ __forceinline__ void mark_tile(const PagesK& p, const int32_t* ref, int tile, int* s) {
+  int n = 0;
+  for (int i = threadIdx.x; i < kTile; i += kThreads) {
+    const int page = tile * kTile + i;
+    const bool fr = page < p.N && ref[page] == 0;
+    const uint64_t b = __ballot(fr);
+    if (threadIdx.x % 32 == 0 && page < p.N) p.bits[page / 32] = (uint32_t)(threadIdx.x % kWave ? b >> 32 : b);
+    n += fr;
+  }
+  n = block_sum(n, s);
+  if (threadIdx.x == 0) p.tfree[tile] = n;
+}
+
+// The free pages of ranks [k0, k0 + n): put(k, page) for each that exists, from
+// the tile counts and the bitmap.  Every thread of the workgroup calls it.
+template <typename Put>
+__device__ __forceinline__ void find_free(const PagesK& p, int k0, int n, int* s, Put put) {
+  int before = 0;
+  for (int t0 = 0; t0 < p.ntiles && before < k0 + n; t0 += kThreads) {
+    const int t = t0 + threadIdx.x;
+    const int c = t < p.ntiles ? p.tfree[t] : 0;
+    int total;
+    const int b = before + block_scan(c, s, &total);
+    // one thread per tile walks its words; the tiles that hold a wanted rank are few
+    if (c > 0 && b < k0 + n && b + c > k0) {
+      int k = b;
+      const int w1 = min((t + 1) * (kTile / 32), (p.N + 31) / 32);
+      for (int w = t * (kTile / 32); w < w1 && k < k0 + n; ++w) {
+        uint32_t x = p.bits[w];
+        const int m = __popc(x);
+        if (k + m <= k0) {
+          k += m;
+          continue;
+        }
+        while (x) {
+          const int bit = __ffs((int)x) - 1;
+          x &= x - 1;
+          if (k >= k0 && k < k0 + n) put(k, w * 32 + bit);
+          ++k;
+        }
+      }
+    }
+    before += total;
+  }
+}
+
+// ---------------------------------------------------------------- reserve
+// rows: the new lengths.  First launch: a workgroup per row copies it and counts
+// what it misses, a workgroup per tile copies ref and counts its free pages.
+__global__ __launch_bounds__(kThreads) void reserve_count_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  if ((int)blockIdx.x < p.R) {
+    const int r = (int)blockIdx.x;
+    const int len = p.rows[r];
+    const int nb = (int)min((int64_t)p.W, ((int64_t)max(len, 0) + p.page_size - 1) / p.page_size);
+    int n = 0;
+    for (int b = threadIdx.x; b < p.W; b += kThreads) {
+      const int id = p.bt[(int64_t)r * p.bt_sr + b];
+      p.bto[(int64_t)r * p.bto_sr + b] = id;
+      n += b < nb && id < 0;
+    }
+    n = block_sum(n, s);
+    if (threadIdx.x == 0) {
+      p.need[r] = n;
+      p.slo[r] = len;
+    }
+  } else {
+    const int tile = (int)blockIdx.x - p.R;
+    for (int i = threadIdx.x; i < kTile; i += kThreads)
+      if (tile * kTile + i < p.N) p.refo[tile * kTile + i] = p.ref[tile * kTile + i];
+    mark_tile(p, p.ref, tile, s);
+  }
+}
+
+// Second launch: each row that misses pages takes the free pages of its ranks.
+__global__ __launch_bounds__(kThreads) void reserve_deal_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  const int r = (int)blockIdx.x;
+  int before = 0, all = 0, fr = 0;
+  const bool last = r == p.R - 1;
+  const int need = p.need[r];
+  if (need == 0 && !last) return;
+  for (int i = threadIdx.x; i < p.R; i += kThreads) {
+    const int n = p.need[i];
+    before += i < r ? n : 0;
+    all += n;
+  }
+  before = block_sum(before, s);
+  if (last) {
+    all = block_sum(all, s);
+    for (int i = threadIdx.x; i < p.ntiles; i += kThreads) fr += p.tfree[i];
+    fr = block_sum(fr, s);
+    if (threadIdx.x == 0) *p.count = max(all - fr, 0);
+    if (need == 0) return;
+  }
+  // the row's missing entries in order: entry of rank k takes the free page of rank before + k
+  const int nb = (int)min((int64_t)p.W, ((int64_t)max(p.rows[r], 0) + p.page_size - 1) / p.page_size);
+  __shared__ int s_blk[kThreads];
+  int done = 0;
+  for (int b0 = 0; b0 < nb && done < need; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    const bool miss = b < nb && p.bt[(int64_t)r * p.bt_sr + b] < 0;
+    int got;
+    const int k = block_scan(miss ? 1 : 0, s, &got);
+    if (miss) s_blk[k] = b;
+    __syncthreads();
+    if (got > 0)
+      find_free(p, before + done, got, s, [&](int rank, int page) {
+        p.bto[(int64_t)r * p.bto_sr + s_blk[rank - before - done]] = page;
+        p.refo[page] = 1;
+      });
+    __syncthreads();
+    done += got;
+  }
+}
+
+// ---------------------------------------------------------------- reorder
+__global__ __launch_bounds__(kThreads) void copy_ref_kernel(PagesK p) {
+  const int i = (int)blockIdx.x * kThreads + threadIdx.x;
+  if (i < p.N) p.refo[i] = p.ref[i];
+}
+
+// rows: the parents.  A workgroup per row writes its new entries, moves the
+// references from its old pages to its new ones and notes the page it must copy.
+__global__ __launch_bounds__(kThreads) void reorder_rows_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  const int r = (int)blockIdx.x;
+  const int par = p.rows[r];
+  const bool alive = par >= 0 && par < p.R;
+  int older = 0;
+  for (int i = threadIdx.x; alive && i < r; i += kThreads) older += p.rows[i] == par;
+  older = block_sum(older, s);
+  const bool first = alive && older == 0;
+  const int len = alive ? p.sl[par] : 0;
+  const int full = max(len, 0) / p.page_size;
+  const int begun = max(len, 0) % p.page_size;
+  for (int b = threadIdx.x; b < p.W; b += kThreads) {
+    const int old = p.bt[(int64_t)r * p.bt_sr + b];
+    const int id = alive ? p.bt[(int64_t)par * p.bt_sr + b] : -1;
+    const bool keep = alive && (first || b < full);
+    const int now = keep ? id : -1;
+    p.bto[(int64_t)r * p.bto_sr + b] = now;
+    if (old != now) {
+      if (valid_page(p, old)) atomicSub(&p.refo[old], 1);
+      if (valid_page(p, now)) atomicAdd(&p.refo[now], 1);
+    }
+  }
+  if (threadIdx.x == 0) {
+    p.slo[r] = len;
+    int src = -1;
+    if (alive && !first && begun > 0 && full < p.W) src = p.bt[(int64_t)par * p.bt_sr + full];
+    p.src[r] = valid_page(p, src) ? src : -1;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void mark_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  mark_tile(p, p.refo, (int)blockIdx.x, s);
+}
+
+// One workgroup deals free pages to the rows that copy, in row order.
+__global__ __launch_bounds__(kThreads) void reorder_deal_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  __shared__ int s_row[kThreads];
+  int fr = 0;
+  for (int i = threadIdx.x; i < p.ntiles; i += kThreads) fr += p.tfree[i];
+  fr = block_sum(fr, s);
+  int done = 0;
+  for (int r0 = 0; r0 < p.R; r0 += kThreads) {
+    const int r = r0 + threadIdx.x;
+    const bool want = r < p.R && p.src[r] >= 0;
+    int n;
+    const int k = block_scan(want ? 1 : 0, s, &n);
+    if (want) s_row[k] = r;
+    if (r < p.R) p.dst[r] = -1;
+    __syncthreads();
+    if (n > 0)
+      find_free(p, done, n, s, [&](int rank, int page) {
+        const int row = s_row[rank - done];
+        p.dst[row] = page;
+        p.bto[(int64_t)row * p.bto_sr + p.slo[row] / p.page_size] = page;
+        p.refo[page] = 1;
+      });
+    __syncthreads();
+    done += n;
+  }
+  if (threadIdx.x == 0) {
+    *p.count = max(done - fr, 0);
+    *p.npairs = p.R;
+  }
+}
+
+// ---------------------------------------------------------------- compact
+__global__ __launch_bounds__(kThreads) void held_count_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  int n = 0;
+  for (int i = threadIdx.x; i < kTile; i += kThreads) {
+    const int page = (int)blockIdx.x * kTile + i;
+    n += page < p.N && p.ref[page] > 0;
+  }
+  n = block_sum(n, s);
+  if (threadIdx.x == 0) p.tfree[blockIdx.x] = n;
+}
+
+// With n pages held, hole number i (the i-th free page below n) takes mover
+// number i (the i-th held page at or past n); there are n - held(< n) of each.
+// Page x is hole x - held(< x) or mover held(< x) - held(< n).
+__global__ __launch_bounds__(kThreads) void compact_plan_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  const int tile = (int)blockIdx.x;
+  int all = 0, before = 0;
+  for (int i = threadIdx.x; i < p.ntiles; i += kThreads) {
+    const int c = p.tfree[i];
+    all += c;
+    before += i < tile ? c : 0;
+  }
+  const int n = block_sum(all, s);
+  before = block_sum(before, s);
+  // held(< n), for the ranks of this tile's movers
+  int below = 0;
+  if ((tile + 1) * kTile >= n) {
+    const int nt = n / kTile;
+    for (int i = threadIdx.x; i < nt; i += kThreads) below += p.tfree[i];
+    for (int i = nt * kTile + threadIdx.x; i < n; i += kThreads) below += p.ref[i] > 0;
+    below = block_sum(below, s);
+  }
+  for (int i0 = 0; i0 < kTile; i0 += kThreads) {
+    const int x = tile * kTile + i0 + threadIdx.x;
+    const bool held = x < p.N && p.ref[x] > 0;
+    int got;
+    const int hb = before + block_scan(held ? 1 : 0, s, &got);   // held pages below x
+    if (x < n && !held) p.dst[x - hb] = x;
+    if (x < p.N && x >= n && held) {
+      p.src[hb - below] = x;
+      p.need[x] = hb - below;
+    }
+    before += got;
+  }
+  if (tile == p.ntiles - 1 && threadIdx.x == 0) {
+    *p.count = n;
+    *p.npairs = n - below;
+  }
+}
+
+// The table follows and the references move (the last workgroups).
+__global__ __launch_bounds__(kThreads) void compact_table_kernel(PagesK p, int row_groups) {
+  const int n = *p.count;
+  if ((int)blockIdx.x < row_groups) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i < (int64_t)p.R * p.W) {
+      const int r = (int)(i / p.W), b = (int)(i % p.W);
+      const int id = p.bt[(int64_t)r * p.bt_sr + b];
+      const bool moves = id >= n && id < p.N && p.ref[id] > 0;
+      p.bto[(int64_t)r * p.bto_sr + b] = moves ? p.dst[p.need[id]] : id;
+    }
+    if (i < p.R) p.slo[i] = p.sl[i];
+  } else {
+    const int x = ((int)blockIdx.x - row_groups) * kThreads + threadIdx.x;
+    if (x < p.N) {
+      const int v = p.ref[x];
+      if (x < n) {
+        if (v > 0) p.refo[x] = v;
+      } else {
+        p.refo[x] = v > 0 ? 0 : v;
+        if (v > 0) p.refo[p.dst[p.need[x]]] = v;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- copy
+struct CopyK {
+  srswa_page_cache c[kMaxCaches];
+  int n;                        // caches
+  const int32_t* src;
+  const int32_t* dst;
+  const int32_t* npairs;
+  int N;
+};
+
+// Workgroups take (pair, cache) items in turn; a pair whose destination is -1
+// copies nothing.  No destination is a source (a source is held, a destination
+// was free), so the order does not matter.
+__global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyK p) {
+  const int64_t items = (int64_t)*p.npairs * p.n;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int i = (int)(it / p.n);
+    const int s = p.src[i], d = p.dst[i];
+    if (s < 0 || s >= p.N || d < 0 || d >= p.N) continue;
+    const srswa_page_cache c = p.c[it % p.n];
+    const unsigned char* from = reinterpret_cast<const unsigned char*>(c.base) + (int64_t)s * c.stride;
+    unsigned char* to = reinterpret_cast<unsigned char*>(c.base) + (int64_t)d * c.stride;
+    const uint64_t al = reinterpret_cast<uintptr_t>(c.base) | (uint64_t)c.stride | (uint64_t)c.bytes;
+    if (al % 16 == 0) {
+      for (int64_t k = threadIdx.x; k < c.bytes / 16; k += kThreads)
+        reinterpret_cast<uint4*>(to)[k] = reinterpret_cast<const uint4*>(from)[k];
+    } else if (al % 4 == 0) {
+      for (int64_t k = threadIdx.x; k < c.bytes / 4; k += kThreads)
+        reinterpret_cast<uint32_t*>(to)[k] = reinterpret_cast<const uint32_t*>(from)[k];
+    } else {
+      for (int64_t k = threadIdx.x; k < c.bytes; k += kThreads) to[k] = from[k];
+    }
+  }
+}
+
+struct Layout {
+  size_t need, src, dst, tfree, npairs, bits, total;
+};
+Layout layout_of(const srswa_pages_args* a) {
+  const size_t n = (size_t)a->num_pages, r = (size_t)a->R, m = std::max(n, r);
+  const size_t tiles = (n + kTile - 1) / kTile;
+  auto up = [](size_t b) { return (b + 63) / 64 * 64; };
+  Layout l;
+  l.need = 0;
+  l.src = l.need + up(m * 4);
+  l.dst = l.src + up(m * 4);
+  l.tfree = l.dst + up(m * 4);
+  l.npairs = l.tfree + up(tiles * 4);
+  l.bits = l.npairs + 64;
+  l.total = l.bits + up((n + 31) / 32 * 4);
+  return l;
+}
+
+int setup(const srswa_pages_args* a, void* ws, size_t ws_bytes, bool rows, const char* what, PagesK* k) {
+  if (!a || !a->block_table || !a->seq_lens || !a->ref || (rows && !a->rows) || !a->block_table_out ||
+      !a->seq_lens_out || !a->ref_out || !a->count || (a->ncaches > 0 && !a->caches)) {
+    set_error("%s: null argument", what);
+    return SRSWA_INVALID;
+  }
+  if (a->R <= 0 || a->W <= 0 || a->num_pages <= 0 || a->page_size <= 0 || a->ncaches < 0) {
+    set_error("%s: bad sizes", what);
+    return SRSWA_INVALID;
+  }
+  if (a->num_pages > (1 << 30) || (int64_t)a->R * a->W > (1ll << 38)) {
+    set_error("%s: more than 2^30 pages or 2^38 table entries", what);
+    return SRSWA_UNSUPPORTED;
+  }
+  for (int i = 0; i < a->ncaches; ++i)
+    if (!a->caches[i].base || a->caches[i].bytes < 0 || a->caches[i].stride < a->caches[i].bytes) {
+      set_error("%s: cache %d is null or its pages overlap", what, i);
+      return SRSWA_INVALID;
+    }
+  const Layout l = layout_of(a);
+  if (!ws || ws_bytes < l.total) {
+    set_error("%s: workspace of %zu bytes required (got %zu)", what, l.total, ws_bytes);
+    return SRSWA_WORKSPACE;
+  }
+  char* w = reinterpret_cast<char*>(ws);
+  *k = PagesK{};
+  k->bt = a->block_table;      k->bt_sr = a->bt_sr;
+  k->sl = a->seq_lens;         k->ref = a->ref;            k->rows = a->rows;
+  k->bto = a->block_table_out; k->bto_sr = a->bto_sr;
+  k->slo = a->seq_lens_out;    k->refo = a->ref_out;       k->count = a->count;
+  k->R = a->R;  k->W = a->W;  k->N = a->num_pages;  k->page_size = a->page_size;
+  k->ntiles = (a->num_pages + kTile - 1) / kTile;
+  k->need = reinterpret_cast<int32_t*>(w + l.need);
+  k->src = reinterpret_cast<int32_t*>(w + l.src);
+  k->dst = reinterpret_cast<int32_t*>(w + l.dst);
+  k->tfree = reinterpret_cast<int32_t*>(w + l.tfree);
+  k->npairs = reinterpret_cast<int32_t*>(w + l.npairs);
+  k->bits = reinterpret_cast<uint32_t*>(w + l.bits);
+  return SRSWA_OK;
+}
+
+void copy_pages(const srswa_pages_args* a, const PagesK& k, int64_t most_pairs, hipStream_t st) {
+  for (int c0 = 0; c0 < a->ncaches; c0 += kMaxCaches) {
+    CopyK c{};
+    c.n = std::min(kMaxCaches, a->ncaches - c0);
+    for (int i = 0; i < c.n; ++i) c.c[i] = a->caches[c0 + i];
+    c.src = k.src;  c.dst = k.dst;  c.npairs = k.npairs;  c.N = k.N;
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most_pairs * c.n, 2048));
+    copy_pages_kernel<<<grid, kThreads, 0, st>>>(c);
+  }
+}
+
+int done(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) {
+    set_error("%s launch failed: %s", what, hipGetErrorString(e));
+    return SRSWA_LAUNCH;
+  }
+  return SRSWA_OK;
+}
+
+}  // namespace
+}  // namespace srswa
+
+using namespace srswa;
+
+extern "C" size_t srswa_pages_workspace(const srswa_pages_args* a) {
+  return a && a->R > 0 && a->num_pages > 0 ? layout_of(a).total : 0;
+}
+
+extern "C" int srswa_pages_reserve(const srswa_pages_args* a, void* ws, size_t ws_bytes, void* stream) {
+  PagesK k;
+  const int rc = setup(a, ws, ws_bytes, true, "pages reserve", &k);
+  if (rc != SRSWA_OK) return rc;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  reserve_count_kernel<<<(unsigned)(k.R + k.ntiles), kThreads, 0, st>>>(k);
+  reserve_deal_kernel<<<(unsigned)k.R, kThreads, 0, st>>>(k);
+  return done("pages reserve");
+}
+
+extern "C" int srswa_pages_reorder(const srswa_pages_args* a, void* ws, size_t ws_bytes, void* stream) {
+  PagesK k;
+  const int rc = setup(a, ws, ws_bytes, true, "pages reorder", &k);
+  if (rc != SRSWA_OK) return rc;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  copy_ref_kernel<<<(unsigned)((k.N + kThreads - 1) / kThreads), kThreads, 0, st>>>(k);
+  reorder_rows_kernel<<<(unsigned)k.R, kThreads, 0, st>>>(k);
+  mark_kernel<<<(unsigned)k.ntiles, kThreads, 0, st>>>(k);
+  reorder_deal_kernel<<<1, kThreads, 0, st>>>(k);
+  copy_pages(a, k, k.R, st);
+  return done("pages reorder");
+}
+
+extern "C" int srswa_pages_compact(const srswa_pages_args* a, void* ws, size_t ws_bytes, void* stream) {
+  PagesK k;
+  const int rc = setup(a, ws, ws_bytes, false, "pages compact", &k);
+  if (rc != SRSWA_OK) return rc;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  held_count_kernel<<<(unsigned)k.ntiles, kThreads, 0, st>>>(k);
+  compact_plan_kernel<<<(unsigned)k.ntiles, kThreads, 0, st>>>(k);
+  const int64_t rows = ((int64_t)k.R * k.W + kThreads - 1) / kThreads;
+  compact_table_kernel<<<(unsigned)(rows + (k.N + kThreads - 1) / kThreads), kThreads, 0, st>>>(k, (int)rows);
+  copy_pages(a, k, k.N / 2 + 1, st);
+  return done("pages compact");
+}

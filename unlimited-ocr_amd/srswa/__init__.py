@@ -9,9 +9,11 @@ from PyTorch-ROCm.  Drop-in modules keep the reference's Python surface:
 * ``srswa.patch``                     -- rebinding of the HF model's decode attend, router
                                          scores / selection, page isolation and Page2D RoPE
 * ``srswa.ops`` / ``srswa.page_ops``  -- the raw operators over the C ABI
+* ``srswa.cache8``                    -- the scaled 8-bit paged cache: append, decode, prefill
+* ``srswa.cache_pages``               -- the pages of a pool: reserve, reorder, compact
 """
 
-from . import _lib  # noqa: F401
+from . import _lib, cache8, cache_pages  # noqa: F401
 from ._lib import UnsupportedShape  # noqa: F401
 from .ops import decode_attend, gather_decode, index_meanpool_topk, topk_rows  # noqa: F401
 

@@ -25,6 +25,7 @@ SRSWA_LAUNCH = 4
 SRSWA_F32 = 0
 SRSWA_BF16 = 1
 SRSWA_F16 = 2
+SRSWA_I8 = 7
 
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -559,6 +560,72 @@ class BmScoreBwdArgs(ctypes.Structure):
     ]
 
 
+class Cache8AppendArgs(ctypes.Structure):
+    """Mirror of ``srswa_cache8_append_args``."""
+
+    _fields_ = [
+        ("k", _vp), ("k_sn", _i64), ("k_sh", _i64),
+        ("v", _vp), ("v_sn", _i64), ("v_sh", _i64),
+        ("k_cache", _vp), ("kc_sp", _i64), ("kc_st", _i64), ("kc_sh", _i64),
+        ("v_cache", _vp), ("vc_sp", _i64), ("vc_st", _i64), ("vc_sh", _i64),
+        ("k_scale", _vp), ("ks_sp", _i64), ("ks_sh", _i64),
+        ("v_scale", _vp), ("vs_sp", _i64), ("vs_sh", _i64),
+        ("block_table", _vp), ("bt_sr", _i64),
+        ("start", _vp),
+        ("cu_seqlens", _vp),
+        ("R", _i32), ("total", _i32), ("max_new_len", _i32), ("HKV", _i32), ("D", _i32), ("max_blocks", _i32),
+        ("num_pages", _i32), ("page_size", _i32),
+        ("dtype", _i32), ("kv_dtype", _i32),
+    ]
+
+
+class Cache8AttendArgs(ctypes.Structure):
+    """Mirror of ``srswa_cache8_attend_args``."""
+
+    _fields_ = [
+        ("q", _vp), ("q_sn", _i64), ("q_sh", _i64),
+        ("k_cache", _vp), ("k_sp", _i64), ("k_st", _i64), ("k_sh", _i64),
+        ("v_cache", _vp), ("v_sp", _i64), ("v_st", _i64), ("v_sh", _i64),
+        ("k_scale", _vp), ("ks_sp", _i64), ("ks_sh", _i64),
+        ("v_scale", _vp), ("vs_sp", _i64), ("vs_sh", _i64),
+        ("block_table", _vp), ("bt_sr", _i64),
+        ("seq_lens", _vp),
+        ("cu_seqlens_q", _vp),
+        ("topk", _vp), ("t_sh", _i64), ("t_sn", _i64), ("t_sk", _i64),
+        ("bias", _vp),
+        ("out", _vp), ("o_sn", _i64), ("o_sh", _i64),
+        ("lse", _vp), ("lse_sn", _i64), ("lse_sh", _i64),
+        ("R", _i32), ("total_q", _i32), ("max_query_len", _i32), ("HQ", _i32), ("HKV", _i32), ("D", _i32),
+        ("topk_n", _i32), ("max_blocks", _i32), ("num_pages", _i32), ("page_size", _i32),
+        ("window", _i32), ("sinks", _i32),
+        ("scale", ctypes.c_float),
+        ("dtype", _i32), ("kv_dtype", _i32),
+    ]
+
+
+class PageCache(ctypes.Structure):
+    """Mirror of ``srswa_page_cache``."""
+
+    _fields_ = [("base", _vp), ("stride", _i64), ("bytes", _i64)]
+
+
+class PagesArgs(ctypes.Structure):
+    """Mirror of ``srswa_pages_args``."""
+
+    _fields_ = [
+        ("block_table", _vp), ("bt_sr", _i64),
+        ("seq_lens", _vp),
+        ("ref", _vp),
+        ("rows", _vp),
+        ("block_table_out", _vp), ("bto_sr", _i64),
+        ("seq_lens_out", _vp),
+        ("ref_out", _vp),
+        ("count", _vp),
+        ("caches", _vp),
+        ("ncaches", _i32), ("R", _i32), ("W", _i32), ("num_pages", _i32), ("page_size", _i32),
+    ]
+
+
 # name -> (restype, argtypes) of every exported entry point
 SIGNATURES = {
     "srswa_version": (ctypes.c_int, []),
@@ -615,6 +682,15 @@ SIGNATURES = {
     "srswa_bm_score_fwd": (ctypes.c_int, [ctypes.POINTER(BmScoreArgs), _vp]),
     "srswa_bm_score_bwd_workspace": (ctypes.c_int, [ctypes.POINTER(BmScoreBwdArgs), _szp]),
     "srswa_bm_score_bwd": (ctypes.c_int, [ctypes.POINTER(BmScoreBwdArgs), _vp, ctypes.c_size_t, _vp]),
+    "srswa_cache8_append": (ctypes.c_int, [ctypes.POINTER(Cache8AppendArgs), _vp]),
+    "srswa_cache8_decode_workspace": (ctypes.c_size_t, [ctypes.POINTER(Cache8AttendArgs)]),
+    "srswa_cache8_decode": (ctypes.c_int, [ctypes.POINTER(Cache8AttendArgs), _vp, ctypes.c_size_t, _vp]),
+    "srswa_cache8_prefill_workspace": (ctypes.c_size_t, [ctypes.POINTER(Cache8AttendArgs)]),
+    "srswa_cache8_prefill": (ctypes.c_int, [ctypes.POINTER(Cache8AttendArgs), _vp, ctypes.c_size_t, _vp]),
+    "srswa_pages_workspace": (ctypes.c_size_t, [ctypes.POINTER(PagesArgs)]),
+    "srswa_pages_reserve": (ctypes.c_int, [ctypes.POINTER(PagesArgs), _vp, ctypes.c_size_t, _vp]),
+    "srswa_pages_reorder": (ctypes.c_int, [ctypes.POINTER(PagesArgs), _vp, ctypes.c_size_t, _vp]),
+    "srswa_pages_compact": (ctypes.c_int, [ctypes.POINTER(PagesArgs), _vp, ctypes.c_size_t, _vp]),
 }
 
 STRUCTS = {"srswa_decode_args": DecodeArgs, "srswa_index_args": IndexArgs,
@@ -634,7 +710,9 @@ STRUCTS = {"srswa_decode_args": DecodeArgs, "srswa_index_args": IndexArgs,
            "srswa_block_bounds_args": BlockBoundsArgs, "srswa_candidate_args": CandidateArgs,
            "srswa_kl_args": KlArgs, "srswa_kl_bwd_args": KlBwdArgs,
            "srswa_hc_score_args": HcScoreArgs, "srswa_hc_score_bwd_args": HcScoreBwdArgs,
-           "srswa_bm_score_args": BmScoreArgs, "srswa_bm_score_bwd_args": BmScoreBwdArgs}
+           "srswa_bm_score_args": BmScoreArgs, "srswa_bm_score_bwd_args": BmScoreBwdArgs,
+           "srswa_cache8_append_args": Cache8AppendArgs, "srswa_cache8_attend_args": Cache8AttendArgs,
+           "srswa_page_cache": PageCache, "srswa_pages_args": PagesArgs}
 
 _lib = None
 _lock = threading.Lock()
@@ -706,6 +784,25 @@ def stream_ptr(device: torch.device) -> int:
             raise ValueError(f"Expected a cuda device, but got: {device}")
         idx = torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(idx)
+
+
+class _Here:
+    """No device to switch to."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one: kernels are launched on
+    a stream of the current device.  Costs nothing where it already is."""
+    return _HERE if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr(t) -> int | None:
