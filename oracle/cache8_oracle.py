@@ -64,9 +64,10 @@ def attend(q, kc, vc, ks, vs, table, cu, lens, scale, window=None, sinks=0, topk
     """q [rows, HQ, D], request r's rows cu[r] .. cu[r + 1) at the end of its
     lens[r] keys.  Returns (o, lse, tol): o, tol [rows, HQ, D], lse [rows, HQ].
 
-    tol bounds a kernel that multiplies in q's type (K) and bf16 (P, V) and sums
-    in fp32: with A = sum p |v| / sum p, every weight may be off by half a bf16
-    step (2^-8) and by twice the logit's error dz, and the sums by n 2^-23; the
+    tol bounds a kernel that multiplies in q's type (K) and fp16 (P, V) and sums
+    in fp32: with A = sum p |v| / sum p, every weight may be off by half an fp16
+    step (2^-11), by twice the logit's error dz and by that of its V scale's
+    logarithm (2^-16 for scales down to 2^-100), and the sums by n 2^-23; the
     output is rounded once more (half a step of its type)."""
     rows, HQ, D = q.shape
     HKV, page, npages = kc.shape[2], kc.shape[1], kc.shape[0]
@@ -115,7 +116,7 @@ def attend(q, kc, vc, ks, vs, table, cu, lens, scale, window=None, sinks=0, topk
                     w = torch.exp(z - lse[i, g])
                     o[i, g] = w @ v
                     a = w @ v.abs()
-                    e = a * (2.0 ** -8 + 2 * dz + (len(at) + 16) * 2.0 ** -23)
+                    e = a * (2.0 ** -11 + 2.0 ** -16 + 2 * dz + (len(at) + 16) * 2.0 ** -23)
                     tol[i, g] = e + half * (o[i, g].abs() + e) + torch.finfo(q.dtype).tiny
     return o, lse, tol
 

@@ -7,7 +7,8 @@
 namespace srswa {
 
 constexpr int kI8 = SRSWA_I8;
-constexpr int kScaleMinExp = -100;   // a page of zeros has scale 2^-100
+constexpr int kScaleMinExp = -100;          // a page of zeros has scale 2^-100
+constexpr float kScaleMin = 0x1p-100f;
 
 template <int KV> constexpr float kQMax = KV == kI8 ? 127.f : 448.f;
 
@@ -60,14 +61,27 @@ __device__ __forceinline__ void from_bytes4(uint32_t w, float* f) {
   }
 }
 
+// two fp32 values -> packed fp16, round to nearest even (v_cvt_pk_f16_f32)
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const f16x2_native_t v = {(_Float16)lo, (_Float16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
 // four bytes -> four values of T, two words (exact: every e4m3 and int8 value
 // is a bf16 and an fp16 value)
 template <int KV, typename T>
 __device__ __forceinline__ uint2 bytes4_to(uint32_t w) {
   if constexpr (KV == kI8) {
-    const float a = i8_f32(w, 0), b = i8_f32(w, 1), c = i8_f32(w, 2), d = i8_f32(w, 3);
-    if constexpr (std::is_same<T, bf16_t>::value) return make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
-    else return make_uint2(pack_h16x2(a, b), pack_h16x2(c, d));
+    if constexpr (std::is_same<T, bf16_t>::value) {
+      return make_uint2(pack_bf16x2(i8_f32(w, 0), i8_f32(w, 1)), pack_bf16x2(i8_f32(w, 2), i8_f32(w, 3)));
+    } else {
+      // x + 128 as a byte b under the exponent of 1024 is the fp16 value 1024 + b
+      const uint32_t u = w ^ 0x80808080u;
+      const f16x2_native_t k = {(_Float16)-1152.f, (_Float16)-1152.f};
+      const f16x2_native_t a = __builtin_bit_cast(f16x2_native_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + k;
+      const f16x2_native_t b = __builtin_bit_cast(f16x2_native_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + k;
+      return make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+    }
   } else {
     return make_uint2(fp8x2_to<KV, T, false>(w), fp8x2_to<KV, T, true>(w));
   }

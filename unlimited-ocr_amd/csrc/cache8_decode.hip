@@ -12,13 +12,17 @@
 //   D layout: lane l holds row l % 16 and keys 4 (l / 16) + 0..3 of each of the
 //         unit's two 16-key groups, which is an A operand of P with its keys in
 //         a fixed order (slot j < 4: group 0, j >= 4: group 1);
-//   O += P V  v_mfma_f32_16x16x32_bf16: a lane loads D / 16 contiguous bytes of
+//   O += P V  v_mfma_f32_16x16x32_f16: a lane loads D / 16 contiguous bytes of
 //         each of its 8 keys (the 16 lanes of a key cover its row), and an 8 x 8
 //         byte transpose by v_perm_b32 gives it the 8 keys of one dim per MFMA.
 // A 16-key group lies in one page (page sizes are multiples of 16), so the K
-// scale joins the softmax scale and the V scale multiplies P, in fp32, before P
-// is rounded to bf16 (2^-9 of each weight; the sum l adds the unrounded ones).
-// The running maximum moves only when a logit exceeds it by 2^8.
+// scale joins the softmax scale, and the V scale joins the exponent: with
+// z' = z + log2 vs, p' = 2^(z' - m) weighs the bytes of V and p' / vs the sum l,
+// so p' needs no range beyond the softmax's own.  p' and V's bytes are multiplied
+// in fp16 whatever q's type is: the bytes are exact there and p' keeps 11 bits
+// (half a step 2^-12; bf16 would lose 2^-9 of each weight).  The running maximum
+// moves only when a z' exceeds it by 2^8 and is kept 2^7 below it, so p' stays
+// below 2^15 and only weights under 2^-31 of the largest vanish.
 // Chunks of one tile are joined by cache8_merge_kernel.
 #include <algorithm>
 
@@ -33,6 +37,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kRows = 16;
+constexpr float kBelow = 7.f, kSlack = 8.f;   // the running maximum's place and play (log2)
 constexpr int kGroup = 16;     // keys per page lookup; a unit is two groups
 
 struct AttendK {
@@ -172,7 +177,7 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
   f32x4_t acc[DV];
 #pragma unroll
   for (int d = 0; d < DV; ++d) acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, msub = 0.f, thr = -INFINITY, l = 0.f;
+  float m = -INFINITY, msub = 0.f, thr = -INFINITY, l = 0.f;   // m: the exponent that p' is relative to
 
   const uint8_t* kcache = reinterpret_cast<const uint8_t*>(a.k_cache) + (int64_t)h * a.k_sh;
   const uint8_t* vcache = reinterpret_cast<const uint8_t*>(a.v_cache) + (int64_t)h * a.v_sh;
@@ -183,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
     // lane i looks up the two groups of this wave's i-th unit from here: first
     // key (-1: nothing to see), page and row in it, scales, bias and bounds
     int dk[2], dpage[2], drow[2], dlo[2], dhi[2];
-    float dks[2], dvs[2], db[2];
+    float dks[2], dvi[2], db[2];
     bool whole = true;
     const int du = u0 + kWaves * lane;
 #pragma unroll
@@ -222,7 +227,9 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
       dpage[e] = ok ? page : 0;
       drow[e] = ok ? key % a.page_size : 0;
       dks[e] = ok ? p.scale_l2 * a.k_scale[(int64_t)page * a.ks_sp + (int64_t)h * a.ks_sh] : 0.f;
-      dvs[e] = ok ? a.v_scale[(int64_t)page * a.vs_sp + (int64_t)h * a.vs_sh] : 0.f;
+      const float vs = ok ? fmaxf(a.v_scale[(int64_t)page * a.vs_sp + (int64_t)h * a.vs_sh], kScaleMin) : 1.f;
+      dvi[e] = 1.f / vs;
+      db[e] += __log2f(vs);
       const int last = key + kGroup - 1;
       if constexpr (SEL)
         whole = whole && ok && key >= dlo[e] && last <= dhi[e] && last < end;
@@ -267,9 +274,9 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dks[e]), i));
-        const float bl = SEL ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(db[e]), i)) : 0.f;
+        const float bl = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(db[e]), i));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[4 * e + j] = SEL ? fmaf(sc[e][j], ks, bl) : sc[e][j] * ks;
+        for (int j = 0; j < 4; ++j) z[4 * e + j] = fmaf(sc[e][j], ks, bl);
       }
       if (!((whole_bits >> i) & 1)) {
         // some key is not visible to some row: its logit is -inf, and a key no
@@ -303,11 +310,11 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
       float zm = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
       if (__any(zm > thr)) {
         zm = xor32_max(xor16_max(zm));
-        const float mn = fmaxf(m, zm);
+        const float mn = fmaxf(m, zm - kBelow);
         const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
         m = mn;
         msub = mn == -INFINITY ? 0.f : mn;
-        thr = mn + 8.f;
+        thr = mn + kBelow + kSlack;
         l *= alpha;
         float ar[4];
 #pragma unroll
@@ -317,17 +324,16 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[d][j] *= ar[j];
       }
-      const float vs0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dvs[0]), i));
-      const float vs1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dvs[1]), i));
+      const float vi0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dvi[0]), i));
+      const float vi1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dvi[1]), i));
       float pe[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         pe[j] = __builtin_amdgcn_exp2f(z[j] - msub);
-        l += pe[j];
-        pe[j] *= j < 4 ? vs0 : vs1;
+        l = fmaf(pe[j], j < 4 ? vi0 : vi1, l);
       }
-      const uint4 pa = make_uint4(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3]), pack_bf16x2(pe[4], pe[5]),
-                                  pack_bf16x2(pe[6], pe[7]));
+      const uint4 pa = make_uint4(pack_f16(pe[0], pe[1]), pack_f16(pe[2], pe[3]), pack_f16(pe[4], pe[5]),
+                                  pack_f16(pe[6], pe[7]));
       // O += P V
 #pragma unroll
       for (int hf = 0; hf < DV / 4; ++hf) {
@@ -341,8 +347,8 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
         transpose4(w[4], w[5], w[6], w[7], tb);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const uint2 x0 = bytes4_to<KV, bf16_t>(ta[d]), x1 = bytes4_to<KV, bf16_t>(tb[d]);
-          acc[4 * hf + d] = mfma16<bf16_t>(pa, make_uint4(x0.x, x0.y, x1.x, x1.y), acc[4 * hf + d]);
+          const uint2 x0 = bytes4_to<KV, __half>(ta[d]), x1 = bytes4_to<KV, __half>(tb[d]);
+          acc[4 * hf + d] = mfma16<__half>(pa, make_uint4(x0.x, x0.y, x1.x, x1.y), acc[4 * hf + d]);
         }
       }
     }
