@@ -87,4 +87,21 @@ __device__ __forceinline__ uint2 bytes4_to(uint32_t w) {
   }
 }
 
+// Host side shared by the two attention forms (cache8_decode.hip): the checks of
+// the arguments, and the split-over-keys form behind both entry points.
+int cache8_check(const srswa_cache8_attend_args* a, const char* what);
+int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream, const char* what);
+size_t cache8_decode_ws(const srswa_cache8_attend_args* a);
+inline bool cache8_plannable(const srswa_cache8_attend_args* a) {
+  return a && a->R > 0 && a->HQ > 0 && a->HKV > 0 && a->page_size >= 16 && a->max_blocks > 0 && a->max_query_len > 0;
+}
+inline int cache8_launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) {
+    set_error("%s launch failed: %s", what, hipGetErrorString(e));
+    return SRSWA_LAUNCH;
+  }
+  return SRSWA_OK;
+}
+
 }  // namespace srswa

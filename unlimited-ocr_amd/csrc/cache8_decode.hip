@@ -442,7 +442,9 @@ __global__ __launch_bounds__(kThreads) void cache8_merge_kernel(AttendK p) {
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int check(const srswa_cache8_attend_args* a, const char* what) {
+}  // namespace
+
+int cache8_check(const srswa_cache8_attend_args* a, const char* what) {
   if (!a || !a->q || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale || !a->block_table || !a->seq_lens ||
       !a->out) {
     set_error("%s: null argument", what);
@@ -492,9 +494,11 @@ int check(const srswa_cache8_attend_args* a, const char* what) {
   return SRSWA_OK;
 }
 
+namespace {
+
 // Chunks: enough workgroups to fill the GPU several times, at least 16 units
 // (four per wave) and at most 64 each, so that requests of uneven length spread.
-AttendK plan(const srswa_cache8_attend_args* a, bool split) {
+AttendK plan(const srswa_cache8_attend_args* a) {
   AttendK p{};
   p.a = *a;
   p.G = a->HQ / a->HKV;
@@ -509,13 +513,9 @@ AttendK plan(const srswa_cache8_attend_args* a, bool split) {
   else if (a->window > 0)
     groups = std::min<int64_t>(groups, ((int64_t)a->window + a->max_query_len) / kGroup + 2 + (a->sinks + kGroup - 1) / kGroup);
   const int64_t units = (groups + 1) / 2;
-  p.upc = 0x7fffffff / 2;
-  p.nchunk = 1;
-  if (split) {
-    const int64_t w = std::max<int64_t>(1, (int64_t)a->R * a->HKV * p.tiles);
-    p.upc = (int)std::min<int64_t>(64, std::max<int64_t>(16, units * w / 4096));
-    p.nchunk = (int)std::max<int64_t>(1, (units + p.upc - 1) / p.upc);
-  }
+  const int64_t w = std::max<int64_t>(1, (int64_t)a->R * a->HKV * p.tiles);
+  p.upc = (int)std::min<int64_t>(64, std::max<int64_t>(16, units * w / 4096));
+  p.nchunk = (int)std::max<int64_t>(1, (units + p.upc - 1) / p.upc);
   return p;
 }
 
@@ -545,11 +545,10 @@ void launch_kv(const AttendK& p, unsigned grid, hipStream_t st) {
   else launch_d<T, kFp8E4M3FN>(p, grid, st);
 }
 
-int run(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream, bool split, const char* what) {
-  const int rc = check(a, what);
-  if (rc != SRSWA_OK) return rc;
-  if (a->R == 0 || a->total_q == 0 || a->max_query_len == 0) return SRSWA_OK;
-  AttendK p = plan(a, split);
+}  // namespace
+
+int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream, const char* what) {
+  AttendK p = plan(a);
   const size_t need = ws_bytes_of(p);
   if (need > 0 && (!ws || ws_bytes < need)) {
     set_error("%s: workspace of %zu bytes required (got %zu)", what, need, ws_bytes);
@@ -564,36 +563,20 @@ int run(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stre
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (a->dtype == SRSWA_BF16) launch_kv<bf16_t>(p, (unsigned)grid, st);
   else launch_kv<__half>(p, (unsigned)grid, st);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) {
-    set_error("%s launch failed: %s", what, hipGetErrorString(e));
-    return SRSWA_LAUNCH;
-  }
-  return SRSWA_OK;
+  return cache8_launched(what);
 }
 
-bool plannable(const srswa_cache8_attend_args* a) {
-  return a && a->R > 0 && a->HQ > 0 && a->HKV > 0 && a->page_size >= 16 && a->max_blocks > 0 && a->max_query_len > 0;
-}
+size_t cache8_decode_ws(const srswa_cache8_attend_args* a) { return ws_bytes_of(plan(a)); }
 
-}  // namespace
 }  // namespace srswa
 
 using namespace srswa;
 
 extern "C" size_t srswa_cache8_decode_workspace(const srswa_cache8_attend_args* a) {
-  return plannable(a) ? ws_bytes_of(plan(a, true)) : 0;
+  return cache8_plannable(a) ? cache8_decode_ws(a) : 0;
 }
 extern "C" int srswa_cache8_decode(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream) {
-  return run(a, ws, ws_bytes, stream, true, "cache8 decode");
-}
-extern "C" size_t srswa_cache8_prefill_workspace(const srswa_cache8_attend_args* a) {
-  return plannable(a) ? ws_bytes_of(plan(a, false)) : 0;
-}
-extern "C" int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream) {
-  if (a && a->topk) {
-    set_error("cache8 prefill: selected blocks are for decode");
-    return SRSWA_UNSUPPORTED;
-  }
-  return run(a, ws, ws_bytes, stream, false, "cache8 prefill");
+  const int rc = cache8_check(a, "cache8 decode");
+  if (rc != SRSWA_OK || !cache8_plannable(a) || a->total_q == 0) return rc;
+  return cache8_decode_run(a, ws, ws_bytes, stream, "cache8 decode");
 }

@@ -1,0 +1,452 @@
+// Attention of many query rows per request over the scaled 8-bit paged cache
+// (gfx950, matrix cores).
+//
+// One workgroup = (request, kv head, tile of 128 rows, part of its keys): four
+// waves of 32 rows, a row being a (token, query head of the group) pair, two
+// workgroups per CU.  Per chunk of 64 keys:
+//   * the chunk's bytes, fetched into registers two chunks ahead, are converted
+//     once for all four waves and stored to LDS, K in q's type and V in fp16
+//     (both exact), into the buffer that the previous chunk does not use: one
+//     barrier per chunk;
+//   * S^T = K Q^T on v_mfma_f32_32x32x16: every lane owns one row and 32 keys;
+//   * a 16-key group lies in one page, so its scales are uniform: z' = scale ks s
+//     + log2 vs - m in one FMA, p' = 2^z' weighs V's bytes, l += p' / vs (see
+//     cache8_decode.hip for the range of p');
+//   * O^T += V^T P^T in fp16, V^T read by ds_read_b64_tr_b16.
+// A chunk that every row of a wave sees whole takes no mask; one that none sees
+// is skipped by the wave.  Parts (few tiles, long keys) write fp32 records that
+// cache8_join_kernel combines.
+#include <algorithm>
+
+#include "cache8.h"
+#include "mfma_common.h"
+
+namespace srswa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRowsWg = 128;
+constexpr int kGroup = 16;
+constexpr int kXcds = 8;
+constexpr float kBelow = 7.f, kSlack = 8.f;
+
+struct PrefillK {
+  srswa_cache8_attend_args a;
+  int G, tiles, nsplit, groups;   // groups = R * HKV * nsplit
+  uint32_t page_mul;              // key / page_size = umulhi(key, page_mul) >> page_shift
+  int page_shift;
+  float scale_l2;
+  float* part;                    // [R * HKV * tiles][nsplit][128 * (D + 2)]
+};
+
+template <int D> struct Lds {
+  static constexpr int KP = D + 8, VP = D + 16;          // row pitches (16-bit elements)
+  static constexpr int kBytes = kChunk * KP * 2, vBytes = kChunk * VP * 2;
+  static constexpr int buf = kBytes + vBytes + 64;       // + four float4 of the groups
+  static constexpr int total = 2 * buf;
+};
+
+struct Tile {
+  int row0, nrows, q0, p0, pmin, pmax, kend, end, c0, c1, chunks;
+};
+
+// What a tile of rows reads: chunks [0, c0) hold the first tokens it sees past
+// its window, chunks c1 .. the rest.
+__device__ __forceinline__ Tile tile_of(const PrefillK& p, int r, int tile) {
+  const srswa_cache8_attend_args& a = p.a;
+  Tile t;
+  const int q0 = min(max(a.cu_seqlens_q[r], 0), a.total_q), q1 = min(max(a.cu_seqlens_q[r + 1], q0), a.total_q);
+  const int ql = min(q1 - q0, a.max_query_len);
+  const int sl = max(a.seq_lens[r], 0);
+  t.q0 = q0;
+  t.p0 = sl - (q1 - q0);
+  t.row0 = tile * kRowsWg;
+  t.nrows = (int)max((int64_t)0, min((int64_t)kRowsWg, (int64_t)ql * p.G - t.row0));
+  t.kend = (int)min((int64_t)sl, (int64_t)a.max_blocks * a.page_size);
+  t.pmin = t.p0 + t.row0 / p.G;
+  t.pmax = t.nrows > 0 ? t.p0 + (t.row0 + t.nrows - 1) / p.G : -1;
+  t.end = min(t.pmax + 1, t.kend);
+  const int lo = a.window > 0 ? max(t.pmin - a.window + 1, 0) : 0;
+  t.c0 = lo > 0 ? (min(min(a.sinks, lo), max(t.end, 0)) + kChunk - 1) / kChunk : 0;
+  t.c1 = max(lo / kChunk, t.c0);
+  t.chunks = t.c0 + max((t.end + kChunk - 1) / kChunk - t.c1, 0);
+  return t;
+}
+
+// Parts of a tile: at least eight chunks each.
+__device__ __forceinline__ int parts_of(const PrefillK& p, const Tile& t) {
+  return max(1, min(p.nsplit, t.chunks / 8));
+}
+
+template <typename T, int KV, int D>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache8_prefill_kernel(PrefillK p) {
+  using L = Lds<D>;
+  constexpr int KP = L::KP, VP = L::VP;
+  constexpr int KS = D / 16, MT = D / 32;
+  constexpr int PPR = D / 16;                    // 16-byte pieces per key row
+  constexpr int NP = kChunk * PPR / kThreads;    // pieces of K (and of V) per thread
+  constexpr int RPP = kThreads / PPR;            // key rows per pass
+  extern __shared__ __align__(16) unsigned char smem[];
+  const srswa_cache8_attend_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int rl = lane & 31, hh = lane >> 5;
+
+  // the hardware deals workgroups to the XCDs in turn: the tiles of one
+  // (request, head, part), which read the same keys, stay on one L2, and the
+  // later, longer tiles come first
+  const int gi = (int)(blockIdx.x % kXcds) + kXcds * (int)(blockIdx.x / kXcds / p.tiles);
+  if (gi >= p.groups) return;
+  const int tile = p.tiles - 1 - (int)(blockIdx.x / kXcds % p.tiles);
+  const int part = gi % p.nsplit, h = gi / p.nsplit % a.HKV, r = gi / p.nsplit / a.HKV;
+  const Tile t = tile_of(p, r, tile);
+  if (t.nrows == 0) return;
+  const int parts = parts_of(p, t);
+  if (part >= parts) return;
+  const int u_lo = (int)((int64_t)t.chunks * part / parts), u_hi = (int)((int64_t)t.chunks * (part + 1) / parts);
+
+  const int wrow = wave * 32 + rl;
+  const int row = t.row0 + min(wrow, t.nrows - 1);
+  const int tok = row / p.G, hq = h * p.G + row % p.G;
+  uint4 qf[KS];
+  {
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(t.q0 + tok) * a.q_sn + (int64_t)hq * a.q_sh + 8 * hh;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + 16 * s);
+  }
+  const int pr = wrow < t.nrows ? t.p0 + tok : -1;
+  const bool wave_live = wave * 32 < t.nrows;
+  const int wpmin = t.p0 + (t.row0 + min(wave * 32, t.nrows - 1)) / p.G;
+  const int wpmax = t.p0 + (t.row0 + min(wave * 32 + 31, t.nrows - 1)) / p.G;
+
+  // staging: piece i of a thread is row tid / PPR + i RPP of the chunk
+  const int srow = tid / PPR, scol = tid % PPR * 16;
+  const bool scales = tid % PPR == 0 && srow % kGroup == 0;    // this thread's pieces begin a 16-key group
+  const int32_t* bt = a.block_table + (int64_t)r * a.bt_sr;
+  const uint8_t* kcache = reinterpret_cast<const uint8_t*>(a.k_cache) + (int64_t)h * a.k_sh + scol;
+  const uint8_t* vcache = reinterpret_cast<const uint8_t*>(a.v_cache) + (int64_t)h * a.v_sh + scol;
+  auto base_of = [&](int u) { return (u < t.c0 ? u : t.c1 + u - t.c0) * kChunk; };
+  int pg[NP];          // page of each piece, looked up one chunk before its bytes
+  uint4 kb[NP], vb[NP];
+  float sk[NP], sv[NP];
+  bool sok[NP];
+  auto lookup = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int key = base_of(u) + srow + i * RPP;
+      pg[i] = -1;
+      if (u < u_hi && key < t.end) pg[i] = bt[__umulhi((uint32_t)key, p.page_mul) >> p.page_shift];
+    }
+  };
+  auto fetch = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int key = base_of(u) + srow + i * RPP;
+      const bool ok = pg[i] >= 0 && pg[i] < a.num_pages;
+      // a key that no row sees is staged as zeros: 0 * NaN would reach O
+      const bool any = ok && (a.window == 0 || key > t.pmin - a.window || key < a.sinks);
+      kb[i] = vb[i] = make_uint4(0u, 0u, 0u, 0u);
+      sok[i] = ok;
+      sk[i] = 0.f;
+      sv[i] = 1.f;
+      if (any) {
+        const int rw = key - (int)(__umulhi((uint32_t)key, p.page_mul) >> p.page_shift) * a.page_size;
+        kb[i] = *reinterpret_cast<const uint4*>(kcache + (int64_t)pg[i] * a.k_sp + (int64_t)rw * a.k_st);
+        vb[i] = *reinterpret_cast<const uint4*>(vcache + (int64_t)pg[i] * a.v_sp + (int64_t)rw * a.v_st);
+      }
+      if (scales && ok) {
+        sk[i] = a.k_scale[(int64_t)pg[i] * a.ks_sp + (int64_t)h * a.ks_sh];
+        sv[i] = a.v_scale[(int64_t)pg[i] * a.vs_sp + (int64_t)h * a.vs_sh];
+      }
+    }
+  };
+  auto stage = [&](int buf) __attribute__((always_inline)) {
+    uint16_t* sK = reinterpret_cast<uint16_t*>(smem + buf * L::buf);
+    uint16_t* sV = reinterpret_cast<uint16_t*>(smem + buf * L::buf + L::kBytes);
+    float4* sg = reinterpret_cast<float4*>(smem + buf * L::buf + L::kBytes + L::vBytes);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int rw = srow + i * RPP;
+      const uint2 k0 = bytes4_to<KV, T>(kb[i].x), k1 = bytes4_to<KV, T>(kb[i].y), k2 = bytes4_to<KV, T>(kb[i].z),
+                  k3 = bytes4_to<KV, T>(kb[i].w);
+      *reinterpret_cast<uint4*>(sK + rw * KP + scol) = make_uint4(k0.x, k0.y, k1.x, k1.y);
+      *reinterpret_cast<uint4*>(sK + rw * KP + scol + 8) = make_uint4(k2.x, k2.y, k3.x, k3.y);
+      const uint2 v0 = bytes4_to<KV, __half>(vb[i].x), v1 = bytes4_to<KV, __half>(vb[i].y),
+                  v2 = bytes4_to<KV, __half>(vb[i].z), v3 = bytes4_to<KV, __half>(vb[i].w);
+      *reinterpret_cast<uint4*>(sV + rw * VP + scol) = make_uint4(v0.x, v0.y, v1.x, v1.y);
+      *reinterpret_cast<uint4*>(sV + rw * VP + scol + 8) = make_uint4(v2.x, v2.y, v3.x, v3.y);
+      if (scales) {
+        const float vs = fmaxf(sv[i], kScaleMin);
+        sg[rw / kGroup] = make_float4(sk[i] * p.scale_l2, __log2f(vs), 1.f / vs, sok[i] ? 1.f : 0.f);
+      }
+    }
+  };
+
+  f32x16_t o[MT];
+#pragma unroll
+  for (int d = 0; d < MT; ++d) o[d] = zero16();
+  float m = -INFINITY, msub = 0.f, thr = -INFINITY, l = 0.f;
+
+  if (u_lo < u_hi) {
+    lookup(u_lo);
+    fetch(u_lo);
+    lookup(u_lo + 1);
+    stage(0);
+    if (u_lo + 1 < u_hi) fetch(u_lo + 1);
+    lookup(u_lo + 2);
+  }
+  __syncthreads();
+  for (int u = u_lo; u < u_hi; ++u) {
+    const int buf = (u - u_lo) & 1;
+    if (u + 1 < u_hi) stage(buf ^ 1);
+    if (u + 2 < u_hi) fetch(u + 2);
+    lookup(u + 3);
+    const uint16_t* sK = reinterpret_cast<const uint16_t*>(smem + buf * L::buf);
+    const uint16_t* sV = reinterpret_cast<const uint16_t*>(smem + buf * L::buf + L::kBytes);
+    const float4* sg = reinterpret_cast<const float4*>(smem + buf * L::buf + L::kBytes + L::vBytes);
+    const int j0 = base_of(u);
+    // wave-uniform: does some row see a key, does every row see every key
+    const bool some = wave_live && j0 <= wpmax && (a.window == 0 || j0 + kChunk - 1 > wpmin - a.window || j0 < a.sinks);
+    if (some) {
+      float4 gs[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) gs[q] = sg[q];
+      const bool whole = j0 + kChunk - 1 <= wpmin && j0 + kChunk <= t.kend &&
+                         (a.window == 0 || j0 > wpmax - a.window || j0 + kChunk <= a.sinks) &&
+                         gs[0].w * gs[1].w * gs[2].w * gs[3].w != 0.f;
+      f32x16_t s[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        s[kt] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          s[kt] = Mfma<T>::mac(*reinterpret_cast<const uint4*>(sK + (32 * kt + rl) * KP + 16 * ks + 8 * hh), qf[ks], s[kt]);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float b = gs[q].y - msub;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[q / 2][8 * (q % 2) + j] = fmaf(s[q / 2][8 * (q % 2) + j], gs[q].x, b);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const int k = j0 + 32 * kt + d_row(x, hh);
+            bool see = k <= pr && k < t.kend && gs[2 * kt + x / 8].w != 0.f;
+            if (a.window > 0) see = see && (k > pr - a.window || k < a.sinks);
+            s[kt][x] = see ? s[kt][x] : -INFINITY;
+          }
+      }
+      float zm = s[0][0];
+#pragma unroll
+      for (int x = 1; x < 16; ++x) zm = fmaxf(zm, s[0][x]);
+#pragma unroll
+      for (int x = 0; x < 16; ++x) zm = fmaxf(zm, s[1][x]);
+      if (__any(zm > thr)) {
+        const float mn = fmaxf(m, xor32_max(zm) + msub - kBelow);
+        const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
+        const float now = mn == -INFINITY ? 0.f : mn, by = msub - now;
+        m = mn;
+        msub = now;
+        thr = mn == -INFINITY ? -INFINITY : kBelow + kSlack;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < MT; ++d)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[d][x] *= alpha;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) s[kt][x] += by;
+      }
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float pe[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            pe[j] = __builtin_amdgcn_exp2f(s[kt][8 * q + j]);
+            l = fmaf(pe[j], gs[2 * kt + q].z, l);
+          }
+          const uint4 pf = make_uint4(pack_f16(pe[0], pe[1]), pack_f16(pe[2], pe[3]), pack_f16(pe[4], pe[5]),
+                                      pack_f16(pe[6], pe[7]));
+#pragma unroll
+          for (int d = 0; d < MT; ++d)
+            o[d] = Mfma<__half>::mac(a_operand_tr<VP>(sV, 32 * kt + 16 * q, 32 * d, lane), pf, o[d]);
+        }
+    }
+    __syncthreads();
+  }
+
+  l = xor32_sum(l);
+  if (!wave_live) return;
+  if (p.nsplit > 1 && parts > 1) {
+    // record: lane-major float4s, then the rows' (m, l)
+    float* rec = p.part + (((int64_t)(r * a.HKV + h) * p.tiles + tile) * p.nsplit + part) * kRowsWg * (D + 2);
+#pragma unroll
+    for (int d = 0; d < MT; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        *reinterpret_cast<float4*>(rec + ((d * 4 + x) * kThreads + tid) * 4) =
+            make_float4(o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]);
+    if (hh == 0) {
+      rec[kRowsWg * D + 2 * wrow] = m;
+      rec[kRowsWg * D + 2 * wrow + 1] = l;
+    }
+    return;
+  }
+  if (wrow >= t.nrows) return;
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + tok) * a.o_sn + (int64_t)hq * a.o_sh + 4 * hh;
+#pragma unroll
+  for (int d = 0; d < MT; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<uint2*>(op + 32 * d + 8 * x) =
+          make_uint2(Mfma<T>::pack2(o[d][4 * x] * inv, o[d][4 * x + 1] * inv),
+                     Mfma<T>::pack2(o[d][4 * x + 2] * inv, o[d][4 * x + 3] * inv));
+  if (a.lse && hh == 0)
+    a.lse[(int64_t)(t.q0 + tok) * a.lse_sn + (int64_t)hq * a.lse_sh] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Joins the parts of a tile, lane by lane as they were written.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void cache8_join_kernel(PrefillK p) {
+  constexpr int MT = D / 32;
+  const srswa_cache8_attend_args& a = p.a;
+  const int tile = (int)blockIdx.x % p.tiles, rh = (int)blockIdx.x / p.tiles, h = rh % a.HKV, r = rh / a.HKV;
+  const Tile t = tile_of(p, r, tile);
+  if (t.nrows == 0) return;
+  const int parts = parts_of(p, t);
+  if (parts == 1) return;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, wrow = wave * 32 + (lane & 31), hh = lane >> 5;
+  if (wrow >= t.nrows) return;
+  const float* rec = p.part + (int64_t)blockIdx.x * p.nsplit * kRowsWg * (D + 2);
+  constexpr int64_t rsz = kRowsWg * (D + 2);
+  float M = -INFINITY, l = 0.f;
+  for (int k = 0; k < parts; ++k) M = fmaxf(M, rec[k * rsz + kRowsWg * D + 2 * wrow]);
+  float4 o[MT * 4];
+#pragma unroll
+  for (int i = 0; i < MT * 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < parts; ++k) {
+    const float mk = rec[k * rsz + kRowsWg * D + 2 * wrow];
+    const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
+    l = fmaf(f, rec[k * rsz + kRowsWg * D + 2 * wrow + 1], l);
+#pragma unroll
+    for (int i = 0; i < MT * 4; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(rec + k * rsz + (i * kThreads + tid) * 4);
+      o[i].x = fmaf(f, x.x, o[i].x); o[i].y = fmaf(f, x.y, o[i].y);
+      o[i].z = fmaf(f, x.z, o[i].z); o[i].w = fmaf(f, x.w, o[i].w);
+    }
+  }
+  const int row = t.row0 + wrow, tok = row / p.G, hq = h * p.G + row % p.G;
+  const float inv = M == -INFINITY ? 0.f : 1.f / l;
+  T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + tok) * a.o_sn + (int64_t)hq * a.o_sh + 4 * hh;
+#pragma unroll
+  for (int i = 0; i < MT * 4; ++i)
+    *reinterpret_cast<uint2*>(op + 32 * (i / 4) + 8 * (i % 4)) =
+        make_uint2(Mfma<T>::pack2(o[i].x * inv, o[i].y * inv), Mfma<T>::pack2(o[i].z * inv, o[i].w * inv));
+  if (a.lse && hh == 0)
+    a.lse[(int64_t)(t.q0 + tok) * a.lse_sn + (int64_t)hq * a.lse_sh] = M == -INFINITY ? -INFINITY : (M + log2f(l)) * kLn2;
+}
+
+// Parts: the fewest that need the least rounds of the GPU per part, where two
+// workgroups share a CU and a (request, head, part)'s tiles an XCD; eight chunks
+// of a full table are one part's least.
+PrefillK plan(const srswa_cache8_attend_args* a) {
+  PrefillK p{};
+  p.a = *a;
+  p.G = a->HQ / a->HKV;
+  p.scale_l2 = a->scale * kLog2e;
+  p.tiles = (int)(((int64_t)a->max_query_len * p.G + kRowsWg - 1) / kRowsWg);
+  int lg = 0;
+  while ((1 << lg) < a->page_size) ++lg;
+  p.page_shift = lg - 1;
+  p.page_mul = (uint32_t)(((1ull << (31 + lg)) / a->page_size) + 1);
+  int64_t keys = (int64_t)a->max_blocks * a->page_size;
+  if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + kRowsWg / p.G + 2 * kChunk + a->sinks);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, keys / kChunk / 8));
+  int cus = device_cu_count();
+  if (cus <= 0) cus = 256;
+  const int64_t slots = std::max(1, cus / kXcds * 2);
+  double best = 1e30;
+  p.nsplit = 1;
+  for (int n = 1; n <= most; ++n) {
+    const int64_t per_xcd = ((int64_t)a->R * a->HKV * n + kXcds - 1) / kXcds * p.tiles;
+    const double cost = (double)((per_xcd + slots - 1) / slots) / n;
+    if (cost < best * 0.95) {
+      best = cost;
+      p.nsplit = n;
+    }
+  }
+  p.groups = a->R * a->HKV * p.nsplit;
+  return p;
+}
+
+size_t ws_bytes_of(const PrefillK& p) {
+  return p.nsplit > 1 ? (size_t)p.groups * p.tiles * kRowsWg * (p.a.D + 2) * sizeof(float) : 0;
+}
+
+// Few rows per request take the form split over the keys.
+bool narrow(const srswa_cache8_attend_args* a) { return (int64_t)a->max_query_len * (a->HQ / a->HKV) <= 32; }
+
+template <typename T, int KV, int D>
+int launch(const PrefillK& p, unsigned grid, hipStream_t st) {
+  static LdsGrant grant;
+  if (!ensure_dynamic_lds(cache8_prefill_kernel<T, KV, D>, Lds<D>::total, &grant)) return SRSWA_LAUNCH;
+  cache8_prefill_kernel<T, KV, D><<<grid, kThreads, Lds<D>::total, st>>>(p);
+  if (p.nsplit > 1)
+    cache8_join_kernel<T, D><<<(unsigned)(p.a.R * p.a.HKV * p.tiles), kThreads, 0, st>>>(p);
+  return SRSWA_OK;
+}
+template <typename T, int KV>
+int launch_d(const PrefillK& p, unsigned grid, hipStream_t st) {
+  return p.a.D == 64 ? launch<T, KV, 64>(p, grid, st) : launch<T, KV, 128>(p, grid, st);
+}
+template <typename T>
+int launch_kv(const PrefillK& p, unsigned grid, hipStream_t st) {
+  return p.a.kv_dtype == SRSWA_I8 ? launch_d<T, kI8>(p, grid, st) : launch_d<T, kFp8E4M3FN>(p, grid, st);
+}
+
+}  // namespace
+}  // namespace srswa
+
+using namespace srswa;
+
+extern "C" size_t srswa_cache8_prefill_workspace(const srswa_cache8_attend_args* a) {
+  if (!cache8_plannable(a)) return 0;
+  return narrow(a) ? cache8_decode_ws(a) : ws_bytes_of(plan(a));
+}
+
+extern "C" int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream) {
+  const char* what = "cache8 prefill";
+  const int rc = cache8_check(a, what);
+  if (rc != SRSWA_OK) return rc;
+  if (a->topk) {
+    set_error("%s: selected blocks are for decode", what);
+    return SRSWA_UNSUPPORTED;
+  }
+  if (!cache8_plannable(a) || a->total_q == 0) return SRSWA_OK;
+  if (!a->cu_seqlens_q) {
+    set_error("%s: cu_seqlens_q is null", what);
+    return SRSWA_INVALID;
+  }
+  if (narrow(a)) return cache8_decode_run(a, ws, ws_bytes, stream, what);
+  PrefillK p = plan(a);
+  const size_t need = ws_bytes_of(p);
+  if (need > 0 && (!ws || ws_bytes < need)) {
+    set_error("%s: workspace of %zu bytes required (got %zu)", what, need, ws_bytes);
+    return SRSWA_WORKSPACE;
+  }
+  p.part = reinterpret_cast<float*>(ws);
+  const int64_t grid = ((int64_t)p.groups + kXcds - 1) / kXcds * kXcds * p.tiles;
+  if (grid > 0x7fffffff || (int64_t)a->R * a->HKV * p.nsplit > 0x7fffffff) {
+    set_error("%s: grid too large", what);
+    return SRSWA_UNSUPPORTED;
+  }
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int ok = a->dtype == SRSWA_BF16 ? launch_kv<bf16_t>(p, (unsigned)grid, st) : launch_kv<__half>(p, (unsigned)grid, st);
+  return ok == SRSWA_OK ? cache8_launched(what) : ok;
+}
