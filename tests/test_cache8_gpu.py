@@ -232,6 +232,9 @@ PREFILL = {
     "wide_group": dict(page=32, HQ=16, HKV=2, D=64, q=[37, 9], ctx=[11, 0], W=2),
     "long_page": dict(page=1024, HQ=1, HKV=1, D=128, q=[100], ctx=[1000], W=2),
     "page48": dict(page=48, HQ=2, HKV=2, D=128, q=[129, 64], ctx=[31, 0], W=4),
+    # few rows, long keys: the keys split over parts, as many as a request has chunks for
+    "parts": dict(page=64, HQ=1, HKV=1, D=128, q=[40, 35], ctx=[2100, 300], W=34),
+    "parts_window": dict(page=16, HQ=2, HKV=1, D=64, q=[33], ctx=[2500], W=160, window=1200, sinks=300),
 }
 
 
@@ -371,6 +374,43 @@ def test_strided_queries_outputs_and_caches(dev):
     cache8.cache8_prefill(*args, torch.tensor([0, 2, 4]).to(dev), torch.tensor(lens).to(dev), 2, scale=0.125,
                           out=wide[:, 2 * H:])
     _check(wide[:, 2 * H:], None, ref, "prefill")
+
+
+def test_ctypes_path_gives_the_same(dev, monkeypatch):
+    """The native host path and the ctypes one (which also converts: 64-bit
+    tables, unordered strides) launch the same work."""
+    from srswa import _lib, cache8, cache_pages
+    assert _lib.host is not None
+    g = torch.Generator().manual_seed(61)
+    page, H, D, lens = 16, 2, 64, [70, 33]
+    table, n = _table(g, lens, page, 5, spare=6)
+    kc, ks = _cache(g, n, page, H, D, E4M3)
+    vc, vs = _cache(g, n, page, H, D, E4M3)
+    q = torch.randn(4, 4, D, generator=g).to(BF).to(dev)
+    x = torch.randn(4, H, D, generator=g).to(BF).to(dev)
+    bt, sl = torch.tensor(table, dtype=torch.int32).to(dev), torch.tensor(lens, dtype=torch.int32).to(dev)
+    ids = torch.randint(-1, 4, (H, 4, 3), generator=g).to(torch.int32).to(dev)
+    ref = torch.zeros(n, dtype=torch.int32, device=dev)
+    ref[bt[bt >= 0].long()] = 1
+    got = []
+    for native in (True, False):
+        wide = not native                                # what only the ctypes path takes
+        if not native:
+            monkeypatch.setattr(_lib, "host", None)
+        c = [t.to(dev).clone() for t in (kc, vc, ks, vs)]
+        b, s = (bt.long(), sl.long()) if wide else (bt, sl)
+        cu = torch.tensor([0, 2, 4], dtype=s.dtype, device=dev)
+        res = [cache8.cache8_decode(q, *c, b, s, scale=0.1, decode_query_len=2, window=20, sinks=3),
+               *cache8.cache8_prefill(q, *c, b, cu, s, 2, scale=0.1, return_lse=True),
+               cache8.decode_selected(q, *c, ids, ids.float(), b, s, decode_query_len=2, local_blocks=1, scale=0.1)]
+        cache8.cache8_append(x, x, *c, b, s - 2, cu_seqlens=cu, max_new_len=2)
+        st, m = cache_pages.pages_reserve(cache_pages.PageTable(bt, sl, ref), s + 3, page_size=page)
+        st, k = cache_pages.pages_reorder(st, torch.tensor([1, 1], device=dev, dtype=s.dtype), c, page_size=page)
+        st, live = cache_pages.pages_compact(st, c)
+        got.append(res + [t.view(torch.int8) for t in c] + list(st) + [m, k, live])
+    assert len(got[0]) == len(got[1])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
 
 
 def test_empty_calls(dev):

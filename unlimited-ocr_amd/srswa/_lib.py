@@ -718,6 +718,18 @@ _lib = None
 _lock = threading.Lock()
 
 
+def _load_host():
+    """The native host path (``_host.so``) of the 8-bit cache and page pool calls,
+    or None where it is not built: the same calls then go through ctypes."""
+    if not os.path.exists(os.path.join(os.path.dirname(os.path.abspath(__file__)), "_host.so")):
+        return None
+    from . import _host
+    return _host
+
+
+host = _load_host()
+
+
 class UnsupportedShape(Exception):
     """The kernels do not cover this shape/dtype (reference contract: caller falls back)."""
 

@@ -80,6 +80,9 @@ def cache8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, 
     key are left as they are.  A page that starts with a new key takes nothing
     from what it held before.  Two requests of one call must not write the same
     page (fork it first: ``cache_pages.pages_reorder``)."""
+    if _lib.host and _lib.host.append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, cu_seqlens,
+                                      max_new_len) is None:
+        return
     dev = _same_device(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, cu_seqlens)
     code, npages, page, HKV, D = _check_cache(k_cache, v_cache, k_scale, v_scale)
     if k.dim() != 3 or k.shape[1:] != (HKV, D) or v.shape != k.shape or v.dtype != k.dtype:
@@ -157,6 +160,8 @@ def _attend_args(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, c
 
 def _window(window, sinks):
     """The kernels' (window, sinks): 0 is no window."""
+    if window is None and sinks == 0:
+        return 0, 0
     w, s = 0 if window is None else int(window), int(sinks)
     if (window is not None and w < 1) or s < 0:
         raise ValueError(f"window {window} (None, or at least the row's own key) / sinks {sinks}")
@@ -182,10 +187,15 @@ def cache8_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, 
     window and the first ``sinks`` keys.  Returns out [rows, HQ, D] in q's dtype
     (0 for a row that sees no key) and, if asked, lse [rows, HQ] (natural log,
     -inf there).  A stored NaN reaches the rows of its request only."""
+    w, s = _window(window, sinks)
+    if _lib.host:
+        got = _lib.host.attend(0, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, None, decode_query_len,
+                               scale, w, s, out, return_lse, None, None)
+        if got is not NotImplemented:
+            return got
     dql = int(decode_query_len)
     if dql < 1 or q.dim() != 3 or q.shape[0] != seq_lens.numel() * dql:
         raise ValueError(f"q {tuple(q.shape)} != {seq_lens.numel()} requests x {dql} rows")
-    w, s = _window(window, sinks)
     a, keep, out, lse, dev = _attend_args(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, None, dql,
                                           scale, w, s, out, return_lse)
     if a.R and a.num_pages and a.max_blocks:
@@ -204,9 +214,14 @@ def cache8_prefill(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlen
     (sizes the grid: later rows of a longer one are not written).  Visibility
     and returns as ``cache8_decode``; rows of q behind the last request are left
     as they are in ``out`` (and unset where ``out`` is not given)."""
+    w, s = _window(window, sinks)
+    if _lib.host:
+        got = _lib.host.attend(1, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens_q,
+                               max_query_len, scale, w, s, out, return_lse, None, None)
+        if got is not NotImplemented:
+            return got
     if q.dim() != 3 or int(max_query_len) < 0:
         raise ValueError(f"q {tuple(q.shape)} / max_query_len {max_query_len}")
-    w, s = _window(window, sinks)
     _same_device(q, cu_seqlens_q)
     cu = _i32(cu_seqlens_q).contiguous()
     if cu.numel() != seq_lens.numel() + 1:
@@ -232,6 +247,12 @@ def decode_selected(q, k_cache, v_cache, k_scale, v_scale, topk_idx, blk_bias, b
     """Block-sparse decode (``ops.gather_decode_paged``) over a scaled cache:
     the window of local_blocks pages, and before it the keys of the listed
     blocks with their slot's bias."""
+    if _lib.host:
+        got = _lib.host.attend(0, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, None, decode_query_len,
+                               scale, min(int(local_blocks) * k_cache.shape[1], _MOST_KEYS), 0, out, False, topk_idx,
+                               blk_bias)
+        if got is not NotImplemented:
+            return got
     _same_device(q, topk_idx, blk_bias)
     dql, total = int(decode_query_len), q.shape[0]
     page, HKV = k_cache.shape[1], k_cache.shape[2]

@@ -31,6 +31,9 @@ class PageTable(NamedTuple):
     ref: torch.Tensor
 
 
+_ENTRIES = {"reserve": 0, "reorder": 1, "compact": 2}
+
+
 def _overlap(x, y):
     """Whether two tensors' memory ranges meet."""
     def span(t):
@@ -55,6 +58,10 @@ def _check(state, what):
 
 
 def _run(entry, state, rows, caches, page_size, out):
+    if out is None and _lib.host:
+        got = _lib.host.pages(_ENTRIES[entry], *state, rows, caches, page_size)
+        if got is not NotImplemented:
+            return PageTable(*got[:3]), got[3]
     name = f"srswa_pages_{entry}"
     _require_cuda(*state, rows, *caches)
     _check(state, name)
