@@ -45,6 +45,12 @@ HIPCC_FLAGS = [
 NO_CONTRACT = {"rope2d.hip", "router.hip", "route_serve.hip"}
 
 
+# Kernels whose matrix-instruction accumulators stay in the vector registers:
+# left to itself the compiler keeps them in the accumulation registers and copies
+# them over and back in every pass of a loop that also rescales them.
+MFMA_VGPRS = {"cache8_decode.hip", "cache8_prefill.hip"}
+
+
 def hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
         if cand and os.path.exists(cand):
@@ -54,6 +60,8 @@ def hipcc() -> str:
 
 def _compile(src: str, obj: str, verbose: bool) -> str:
     extra = ["-ffp-contract=off"] if os.path.basename(src) in NO_CONTRACT else []
+    if os.path.basename(src) in MFMA_VGPRS:
+        extra += ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
     cmd = [hipcc(), *HIPCC_FLAGS, *extra, "-c", src, "-o", obj]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -61,6 +61,24 @@ __device__ __forceinline__ void from_bytes4(uint32_t w, float* f) {
   }
 }
 
+// A wave-uniform condition in a form the compiler must take for a lane's own, so
+// that the rare updates under it happen in place: under a uniform branch it copied
+// the whole set of accumulators to other registers on the common path.
+__device__ __forceinline__ bool per_lane(bool c) {
+  int v = c;
+  asm("" : "+v"(v));
+  return v != 0;
+}
+
+// Waits here for loaded values that a loop uses: left alone, the wait stands at
+// their first use inside the loop and, counting in order, drains the loop's own
+// prefetches in every pass.
+template <int N>
+__device__ __forceinline__ void settle(uint4 (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i].x), "+v"(v[i].y), "+v"(v[i].z), "+v"(v[i].w));
+}
+
 // two fp32 values -> packed fp16, round to nearest even (v_cvt_pk_f16_f32)
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const f16x2_native_t v = {(_Float16)lo, (_Float16)hi};

@@ -238,6 +238,7 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
                 (a.window == 0 || key > t.pmax - a.window || last < a.sinks);
     }
     const uint64_t whole_bits = __ballot(whole);
+    settle(qf);
     const int cnt = min(kWave, (u_end - u0 + kWaves - 1) / kWaves);
 
     auto load = [&](int i, UnitBytes<D>& b) __attribute__((always_inline)) {
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) z[4 * e + j] = fmaf(sc[e][j], ks, bl);
       }
-      if (!((whole_bits >> i) & 1)) {
+      if (per_lane(!((whole_bits >> i) & 1))) {
         // some key is not visible to some row: its logit is -inf, and a key no
         // row sees has its V bytes cleared (0 * NaN would reach O)
 #pragma unroll
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
         }
       }
       float zm = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
-      if (__any(zm > thr)) {
+      if (per_lane(__any(zm > thr))) {
         zm = xor32_max(xor16_max(zm));
         const float mn = fmaxf(m, zm - kBelow);
         const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
@@ -479,10 +480,14 @@ int cache8_check(const srswa_cache8_attend_args* a, const char* what) {
     }
   const int64_t ks[] = {a->k_sp, a->k_st, a->k_sh, a->v_sp, a->v_st, a->v_sh};
   for (int64_t s : ks)
-    if (s % 16) {
-      set_error("%s: cache strides must keep rows 16-byte aligned", what);
+    if (s % 16 || s < 0 || s > INT32_MAX) {
+      set_error("%s: cache strides must keep rows 16-byte aligned and be below 2^31", what);
       return SRSWA_UNSUPPORTED;
     }
+  if (a->ks_sp < 0 || a->ks_sp > INT32_MAX || a->vs_sp < 0 || a->vs_sp > INT32_MAX) {
+    set_error("%s: scale strides must be below 2^31", what);
+    return SRSWA_UNSUPPORTED;
+  }
   if (!al16(a->q) || !al16(a->k_cache) || !al16(a->v_cache) || !al16(a->out)) {
     set_error("%s: pointers must be 16-byte aligned", what);
     return SRSWA_UNSUPPORTED;

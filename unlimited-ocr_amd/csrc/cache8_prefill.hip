@@ -36,11 +36,15 @@ struct PrefillK {
   uint32_t page_mul;              // key / page_size = umulhi(key, page_mul) >> page_shift
   int page_shift;
   float scale_l2;
+  bool by_group;                  // the tiles of a group to one XCD, else in turn
   float* part;                    // [R * HKV * tiles][nsplit][128 * (D + 2)]
 };
 
 template <int D> struct Lds {
-  static constexpr int KP = D + 8, VP = D + 16;          // row pitches (16-bit elements)
+  // row pitches (16-bit elements): K rows 4 banks apart, so 16 lanes' 16 bytes of
+  // 16 rows meet no bank twice; V rows 16 banks (of 64) apart, so the two 16-lane
+  // groups of a transposing read (4 rows x 64 bytes) do not either
+  static constexpr int KP = D + 8, VP = D + 32;
   static constexpr int kBytes = kChunk * KP * 2, vBytes = kChunk * VP * 2;
   static constexpr int buf = kBytes + vBytes + 64;       // + four float4 of the groups
   static constexpr int total = 2 * buf;
@@ -73,17 +77,23 @@ __device__ __forceinline__ Tile tile_of(const PrefillK& p, int r, int tile) {
   return t;
 }
 
+// c + the sum of a packed fp16 pair
+__device__ __forceinline__ float dot2_ones(uint32_t w, float c) {
+  const f16x2_native_t one = {(_Float16)1.f, (_Float16)1.f};
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_native_t, w), one, c, false);
+}
+
 // Parts of a tile: at least eight chunks each.
 __device__ __forceinline__ int parts_of(const PrefillK& p, const Tile& t) {
   return max(1, min(p.nsplit, t.chunks / 8));
 }
 
-template <typename T, int KV, int D>
+template <typename T, int KV, int D, bool ONE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache8_prefill_kernel(PrefillK p) {
   using L = Lds<D>;
   constexpr int KP = L::KP, VP = L::VP;
   constexpr int KS = D / 16, MT = D / 32;
-  constexpr int PPR = D / 16;                    // 16-byte pieces per key row
+  constexpr int PPR = D / 8;                     // 8-byte pieces per key row
   constexpr int NP = kChunk * PPR / kThreads;    // pieces of K (and of V) per thread
   constexpr int RPP = kThreads / PPR;            // key rows per pass
   extern __shared__ __align__(16) unsigned char smem[];
@@ -91,12 +101,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int rl = lane & 31, hh = lane >> 5;
 
-  // the hardware deals workgroups to the XCDs in turn: the tiles of one
-  // (request, head, part), which read the same keys, stay on one L2, and the
-  // later, longer tiles come first
-  const int gi = (int)(blockIdx.x % kXcds) + kXcds * (int)(blockIdx.x / kXcds / p.tiles);
-  if (gi >= p.groups) return;
-  const int tile = p.tiles - 1 - (int)(blockIdx.x / kXcds % p.tiles);
+  // The hardware deals workgroups to the XCDs in turn.  One request: the tiles of
+  // one (head, part), which read the same keys, stay on one XCD's L2.  Several: their
+  // lengths are known on the device only, so consecutive workgroups take one tile
+  // of each (request, head, part), which spreads every length over the XCDs.
+  // Later, longer tiles come first.
+  int gi, tile;
+  if (p.by_group) {
+    gi = (int)(blockIdx.x % kXcds) + kXcds * (int)(blockIdx.x / kXcds / p.tiles);
+    if (gi >= p.groups) return;
+    tile = p.tiles - 1 - (int)(blockIdx.x / kXcds % p.tiles);
+  } else {
+    gi = (int)(blockIdx.x % p.groups);
+    tile = p.tiles - 1 - (int)(blockIdx.x / p.groups);
+  }
   const int part = gi % p.nsplit, h = gi / p.nsplit % a.HKV, r = gi / p.nsplit / a.HKV;
   const Tile t = tile_of(p, r, tile);
   if (t.nrows == 0) return;
@@ -118,66 +136,98 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int wpmin = t.p0 + (t.row0 + min(wave * 32, t.nrows - 1)) / p.G;
   const int wpmax = t.p0 + (t.row0 + min(wave * 32 + 31, t.nrows - 1)) / p.G;
 
-  // staging: piece i of a thread is row tid / PPR + i RPP of the chunk
-  const int srow = tid / PPR, scol = tid % PPR * 16;
-  const bool scales = tid % PPR == 0 && srow % kGroup == 0;    // this thread's pieces begin a 16-key group
-  const int32_t* bt = a.block_table + (int64_t)r * a.bt_sr;
-  const uint8_t* kcache = reinterpret_cast<const uint8_t*>(a.k_cache) + (int64_t)h * a.k_sh + scol;
-  const uint8_t* vcache = reinterpret_cast<const uint8_t*>(a.v_cache) + (int64_t)h * a.v_sh + scol;
+  // staging: piece i of a thread is 8 bytes of row srow + i RPP of the chunk.  A
+  // wave's rows of one pass lie in one 16-key group, so its page and the address
+  // of the group's first row are scalar, and a lane adds a constant offset.  Every
+  // load is unconditional, from clamped pages and keys (a branch around one would
+  // have its registers waited for where the paths meet); what no row may see is
+  // zeroed as it is stored, for 0 * NaN would reach O.
+  const int srow = tid / PPR, scol = tid % PPR * 8;
+  const int wgrp = wave * kWave / PPR / kGroup;                     // the wave's group in pass 0
+  const uint32_t koff = (uint32_t)(srow - wgrp * kGroup) * (uint32_t)a.k_st + scol;
+  const uint32_t voff = (uint32_t)(srow - wgrp * kGroup) * (uint32_t)a.v_st + scol;
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+  const scalar_ints bt = (scalar_ints)(a.block_table + (int64_t)r * a.bt_sr);
+  const uint8_t* kcache = reinterpret_cast<const uint8_t*>(a.k_cache) + (int64_t)h * a.k_sh;
+  const uint8_t* vcache = reinterpret_cast<const uint8_t*>(a.v_cache) + (int64_t)h * a.v_sh;
+  const float *kscale = a.k_scale + (int64_t)h * a.ks_sh, *vscale = a.v_scale + (int64_t)h * a.vs_sh;
   auto base_of = [&](int u) { return (u < t.c0 ? u : t.c1 + u - t.c0) * kChunk; };
-  int pg[NP];          // page of each piece, looked up one chunk before its bytes
-  uint4 kb[NP], vb[NP];
-  float sk[NP], sv[NP];
-  bool sok[NP];
+  auto block_of = [&](int key) { return (int)(__umulhi((uint32_t)key, p.page_mul) >> p.page_shift); };
+  // ONE: pages of a multiple of 64 keys hold whole chunks, one lookup each (the
+  // scalar address arithmetic of four took as long as the conversions: 2,048 rows
+  // after 30,720 keys 555 -> 470 us); else one lookup per 16-key group
+  constexpr int NG = ONE ? 1 : 4;
+  auto of_lane = [&](const int (&v)[NG]) {
+    if constexpr (ONE) return v[0];
+    else return tid & 2 ? (tid & 1 ? v[3] : v[2]) : (tid & 1 ? v[1] : v[0]);
+  };
+  auto of_piece = [&](const int (&v)[NG], int i) {                  // the entry of piece i's group
+    if constexpr (ONE) return v[0];
+    else return D == 128 ? v[i] : (wgrp ? v[1 + 2 * i] : v[2 * i]);
+  };
+  auto offset = [](int n, int64_t stride) { return (uint64_t)(uint32_t)n * (uint32_t)stride; };   // (strides below 2^31)
+  int pgn[NG], pgs[NG];              // page ids of the groups: of the chunk to fetch, of the chunk to stage
+  uint2 kb[NP], vb[NP];
+  float gk, gv;                      // the scales of group tid % 4
   auto lookup = [&](int u) __attribute__((always_inline)) {
+    const int j = base_of(min(u, u_hi - 1));
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int key = base_of(u) + srow + i * RPP;
-      pg[i] = -1;
-      if (u < u_hi && key < t.end) pg[i] = bt[__umulhi((uint32_t)key, p.page_mul) >> p.page_shift];
-    }
+    for (int q = 0; q < NG; ++q) pgn[q] = bt[block_of(min(j + q * kGroup, t.end - 1))];
   };
   auto fetch = [&](int u) __attribute__((always_inline)) {
+    const int j = base_of(min(u, u_hi - 1));
+    int safe[NG];
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      pgs[q] = pgn[q];
+      safe[q] = pgn[q] >= 0 && pgn[q] < a.num_pages ? pgn[q] : 0;
+    }
+    const int gp = of_lane(safe);
+    gk = kscale[offset(gp, a.ks_sp)];
+    gv = vscale[offset(gp, a.vs_sp)];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int key = base_of(u) + srow + i * RPP;
-      const bool ok = pg[i] >= 0 && pg[i] < a.num_pages;
-      // a key that no row sees is staged as zeros: 0 * NaN would reach O
-      const bool any = ok && (a.window == 0 || key > t.pmin - a.window || key < a.sinks);
-      kb[i] = vb[i] = make_uint4(0u, 0u, 0u, 0u);
-      sok[i] = ok;
-      sk[i] = 0.f;
-      sv[i] = 1.f;
-      if (any) {
-        const int rw = key - (int)(__umulhi((uint32_t)key, p.page_mul) >> p.page_shift) * a.page_size;
-        kb[i] = *reinterpret_cast<const uint4*>(kcache + (int64_t)pg[i] * a.k_sp + (int64_t)rw * a.k_st);
-        vb[i] = *reinterpret_cast<const uint4*>(vcache + (int64_t)pg[i] * a.v_sp + (int64_t)rw * a.v_st);
-      }
-      if (scales && ok) {
-        sk[i] = a.k_scale[(int64_t)pg[i] * a.ks_sp + (int64_t)h * a.ks_sh];
-        sv[i] = a.v_scale[(int64_t)pg[i] * a.vs_sp + (int64_t)h * a.vs_sh];
-      }
+      const int q = D == 128 ? i : wgrp + 2 * i;                    // RPP is 16 or 32 rows
+      const int key = ONE ? j : min(j + q * kGroup, t.end - 1) & ~(kGroup - 1);
+      const int page = of_piece(safe, i), rw = key - block_of(key) * a.page_size + (ONE ? q * kGroup : 0);
+      kb[i] = *reinterpret_cast<const uint2*>(kcache + (offset(page, a.k_sp) + offset(rw, a.k_st)) + koff);
+      vb[i] = *reinterpret_cast<const uint2*>(vcache + (offset(page, a.v_sp) + offset(rw, a.v_st)) + voff);
     }
   };
-  auto stage = [&](int buf) __attribute__((always_inline)) {
-    uint16_t* sK = reinterpret_cast<uint16_t*>(smem + buf * L::buf);
-    uint16_t* sV = reinterpret_cast<uint16_t*>(smem + buf * L::buf + L::kBytes);
-    float4* sg = reinterpret_cast<float4*>(smem + buf * L::buf + L::kBytes + L::vBytes);
+  auto stage = [&](int u, int buf) __attribute__((always_inline)) {
+    const int j = base_of(u);
+    int ok[NG];
+    bool inside = j + kChunk <= t.end && (a.window == 0 || j > t.pmin - a.window || j + kChunk <= a.sinks);
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      ok[q] = pgs[q] >= 0 && pgs[q] < a.num_pages && j + q * kGroup < t.end;
+      inside = inside && ok[q];
+    }
+    if (per_lane(!inside)) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int key = j + srow + i * RPP;
+        const bool any = of_piece(ok, i) && key < t.end && (a.window == 0 || key > t.pmin - a.window || key < a.sinks);
+        kb[i].x = any ? kb[i].x : 0u;
+        kb[i].y = any ? kb[i].y : 0u;
+        vb[i].x = any ? vb[i].x : 0u;
+        vb[i].y = any ? vb[i].y : 0u;
+      }
+    }
+    uint16_t* sK = reinterpret_cast<uint16_t*>(smem + buf * L::buf) + srow * KP + scol;
+    uint16_t* sV = reinterpret_cast<uint16_t*>(smem + buf * L::buf + L::kBytes) + srow * VP + scol;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int rw = srow + i * RPP;
-      const uint2 k0 = bytes4_to<KV, T>(kb[i].x), k1 = bytes4_to<KV, T>(kb[i].y), k2 = bytes4_to<KV, T>(kb[i].z),
-                  k3 = bytes4_to<KV, T>(kb[i].w);
-      *reinterpret_cast<uint4*>(sK + rw * KP + scol) = make_uint4(k0.x, k0.y, k1.x, k1.y);
-      *reinterpret_cast<uint4*>(sK + rw * KP + scol + 8) = make_uint4(k2.x, k2.y, k3.x, k3.y);
-      const uint2 v0 = bytes4_to<KV, __half>(vb[i].x), v1 = bytes4_to<KV, __half>(vb[i].y),
-                  v2 = bytes4_to<KV, __half>(vb[i].z), v3 = bytes4_to<KV, __half>(vb[i].w);
-      *reinterpret_cast<uint4*>(sV + rw * VP + scol) = make_uint4(v0.x, v0.y, v1.x, v1.y);
-      *reinterpret_cast<uint4*>(sV + rw * VP + scol + 8) = make_uint4(v2.x, v2.y, v3.x, v3.y);
-      if (scales) {
-        const float vs = fmaxf(sv[i], kScaleMin);
-        sg[rw / kGroup] = make_float4(sk[i] * p.scale_l2, __log2f(vs), 1.f / vs, sok[i] ? 1.f : 0.f);
-      }
+      const uint2 k0 = bytes4_to<KV, T>(kb[i].x), k1 = bytes4_to<KV, T>(kb[i].y);
+      *reinterpret_cast<uint4*>(sK + i * RPP * KP) = make_uint4(k0.x, k0.y, k1.x, k1.y);
+      const uint2 v0 = bytes4_to<KV, __half>(vb[i].x), v1 = bytes4_to<KV, __half>(vb[i].y);
+      *reinterpret_cast<uint4*>(sV + i * RPP * VP) = make_uint4(v0.x, v0.y, v1.x, v1.y);
+    }
+    if (tid < 4) {
+      const bool good = of_lane(ok) != 0;
+      const float vs = good ? fmaxf(gv, kScaleMin) : 1.f;
+      reinterpret_cast<float4*>(smem + buf * L::buf + L::kBytes + L::vBytes)[tid] =
+          make_float4(good ? gk * p.scale_l2 : 0.f, __log2f(vs), __builtin_amdgcn_rcpf(vs), good ? 1.f : 0.f);
     }
   };
 
@@ -190,15 +240,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     lookup(u_lo);
     fetch(u_lo);
     lookup(u_lo + 1);
-    stage(0);
-    if (u_lo + 1 < u_hi) fetch(u_lo + 1);
+    stage(u_lo, 0);
+    fetch(u_lo + 1);
     lookup(u_lo + 2);
   }
+  settle(qf);
   __syncthreads();
   for (int u = u_lo; u < u_hi; ++u) {
     const int buf = (u - u_lo) & 1;
-    if (u + 1 < u_hi) stage(buf ^ 1);
-    if (u + 2 < u_hi) fetch(u + 2);
+    stage(min(u + 1, u_hi - 1), buf ^ 1);
+    fetch(u + 2);
     lookup(u + 3);
     const uint16_t* sK = reinterpret_cast<const uint16_t*>(smem + buf * L::buf);
     const uint16_t* sV = reinterpret_cast<const uint16_t*>(smem + buf * L::buf + L::kBytes);
@@ -227,7 +278,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[q / 2][8 * (q % 2) + j] = fmaf(s[q / 2][8 * (q % 2) + j], gs[q].x, b);
       }
-      if (!whole) {
+      if (per_lane(!whole)) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -243,7 +294,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       for (int x = 1; x < 16; ++x) zm = fmaxf(zm, s[0][x]);
 #pragma unroll
       for (int x = 0; x < 16; ++x) zm = fmaxf(zm, s[1][x]);
-      if (__any(zm > thr)) {
+      if (per_lane(__any(zm > thr))) {
         const float mn = fmaxf(m, xor32_max(zm) + msub - kBelow);
         const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
         const float now = mn == -INFINITY ? 0.f : mn, by = msub - now;
@@ -264,14 +315,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          float pe[8];
+          float pe[8], sum;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            pe[j] = __builtin_amdgcn_exp2f(s[kt][8 * q + j]);
-            l = fmaf(pe[j], gs[2 * kt + q].z, l);
-          }
+          for (int j = 0; j < 8; ++j) pe[j] = __builtin_amdgcn_exp2f(s[kt][8 * q + j]);
           const uint4 pf = make_uint4(pack_f16(pe[0], pe[1]), pack_f16(pe[2], pe[3]), pack_f16(pe[4], pe[5]),
                                       pack_f16(pe[6], pe[7]));
+          sum = dot2_ones(pf.w, dot2_ones(pf.z, dot2_ones(pf.y, dot2_ones(pf.x, 0.f))));   // of the rounded weights
+          l = fmaf(sum, gs[2 * kt + q].z, l);
 #pragma unroll
           for (int d = 0; d < MT; ++d)
             o[d] = Mfma<__half>::mac(a_operand_tr<VP>(sV, 32 * kt + 16 * q, 32 * d, lane), pf, o[d]);
@@ -311,44 +361,46 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     a.lse[(int64_t)(t.q0 + tok) * a.lse_sn + (int64_t)hq * a.lse_sh] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// Joins the parts of a tile, lane by lane as they were written.
+// Joins the parts of a tile, lane by lane as they were written: one workgroup per
+// 32 rows, D / 32 x 64 threads of 16 dims each.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void cache8_join_kernel(PrefillK p) {
-  constexpr int MT = D / 32;
+__global__ __launch_bounds__(2 * D) void cache8_join_kernel(PrefillK p) {
   const srswa_cache8_attend_args& a = p.a;
-  const int tile = (int)blockIdx.x % p.tiles, rh = (int)blockIdx.x / p.tiles, h = rh % a.HKV, r = rh / a.HKV;
+  const int wave = (int)blockIdx.x % 4, rt = (int)blockIdx.x / 4;     // the wave that wrote the rows
+  const int tile = rt % p.tiles, rh = rt / p.tiles, h = rh % a.HKV, r = rh / a.HKV;
   const Tile t = tile_of(p, r, tile);
-  if (t.nrows == 0) return;
   const int parts = parts_of(p, t);
-  if (parts == 1) return;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, wrow = wave * 32 + (lane & 31), hh = lane >> 5;
-  if (wrow >= t.nrows) return;
-  const float* rec = p.part + (int64_t)blockIdx.x * p.nsplit * kRowsWg * (D + 2);
+  if (wave * 32 >= t.nrows || parts == 1) return;
+  const int lane = threadIdx.x % kWave, d = threadIdx.x / kWave, wrow = wave * 32 + (lane & 31), hh = lane >> 5;
   constexpr int64_t rsz = kRowsWg * (D + 2);
+  const float* rec = p.part + (int64_t)rt * p.nsplit * rsz;
+  const float* ml = rec + kRowsWg * D + 2 * wrow;
   float M = -INFINITY, l = 0.f;
-  for (int k = 0; k < parts; ++k) M = fmaxf(M, rec[k * rsz + kRowsWg * D + 2 * wrow]);
-  float4 o[MT * 4];
+  for (int k = 0; k < parts; ++k) M = fmaxf(M, ml[k * rsz]);
+  float4 o[4];
 #pragma unroll
-  for (int i = 0; i < MT * 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
   for (int k = 0; k < parts; ++k) {
-    const float mk = rec[k * rsz + kRowsWg * D + 2 * wrow];
+    const float mk = ml[k * rsz];
     const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
-    l = fmaf(f, rec[k * rsz + kRowsWg * D + 2 * wrow + 1], l);
+    l = fmaf(f, ml[k * rsz + 1], l);
 #pragma unroll
-    for (int i = 0; i < MT * 4; ++i) {
-      const float4 x = *reinterpret_cast<const float4*>(rec + k * rsz + (i * kThreads + tid) * 4);
+    for (int i = 0; i < 4; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(rec + k * rsz + ((d * 4 + i) * kThreads + wave * kWave + lane) * 4);
       o[i].x = fmaf(f, x.x, o[i].x); o[i].y = fmaf(f, x.y, o[i].y);
       o[i].z = fmaf(f, x.z, o[i].z); o[i].w = fmaf(f, x.w, o[i].w);
     }
   }
+  if (wrow >= t.nrows) return;
   const int row = t.row0 + wrow, tok = row / p.G, hq = h * p.G + row % p.G;
   const float inv = M == -INFINITY ? 0.f : 1.f / l;
-  T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + tok) * a.o_sn + (int64_t)hq * a.o_sh + 4 * hh;
+  T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + tok) * a.o_sn + (int64_t)hq * a.o_sh + 32 * d + 4 * hh;
 #pragma unroll
-  for (int i = 0; i < MT * 4; ++i)
-    *reinterpret_cast<uint2*>(op + 32 * (i / 4) + 8 * (i % 4)) =
-        make_uint2(Mfma<T>::pack2(o[i].x * inv, o[i].y * inv), Mfma<T>::pack2(o[i].z * inv, o[i].w * inv));
-  if (a.lse && hh == 0)
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<uint2*>(op + 8 * i) = make_uint2(Mfma<T>::pack2(o[i].x * inv, o[i].y * inv),
+                                                       Mfma<T>::pack2(o[i].z * inv, o[i].w * inv));
+  if (a.lse && hh == 0 && d == 0)
     a.lse[(int64_t)(t.q0 + tok) * a.lse_sn + (int64_t)hq * a.lse_sh] = M == -INFINITY ? -INFINITY : (M + log2f(l)) * kLn2;
 }
 
@@ -382,6 +434,7 @@ PrefillK plan(const srswa_cache8_attend_args* a) {
     }
   }
   p.groups = a->R * a->HKV * p.nsplit;
+  p.by_group = a->R == 1;
   return p;
 }
 
@@ -392,13 +445,20 @@ size_t ws_bytes_of(const PrefillK& p) {
 // Few rows per request take the form split over the keys.
 bool narrow(const srswa_cache8_attend_args* a) { return (int64_t)a->max_query_len * (a->HQ / a->HKV) <= 32; }
 
+template <typename T, int KV, int D, bool ONE>
+int launch_tiles(const PrefillK& p, unsigned grid, hipStream_t st) {
+  static LdsGrant grant;
+  if (!ensure_dynamic_lds(cache8_prefill_kernel<T, KV, D, ONE>, Lds<D>::total, &grant)) return SRSWA_LAUNCH;
+  cache8_prefill_kernel<T, KV, D, ONE><<<grid, kThreads, Lds<D>::total, st>>>(p);
+  return SRSWA_OK;
+}
 template <typename T, int KV, int D>
 int launch(const PrefillK& p, unsigned grid, hipStream_t st) {
-  static LdsGrant grant;
-  if (!ensure_dynamic_lds(cache8_prefill_kernel<T, KV, D>, Lds<D>::total, &grant)) return SRSWA_LAUNCH;
-  cache8_prefill_kernel<T, KV, D><<<grid, kThreads, Lds<D>::total, st>>>(p);
+  const int rc = p.a.page_size % kChunk == 0 ? launch_tiles<T, KV, D, true>(p, grid, st)
+                                             : launch_tiles<T, KV, D, false>(p, grid, st);
+  if (rc != SRSWA_OK) return rc;
   if (p.nsplit > 1)
-    cache8_join_kernel<T, D><<<(unsigned)(p.a.R * p.a.HKV * p.tiles), kThreads, 0, st>>>(p);
+    cache8_join_kernel<T, D><<<(unsigned)(p.a.R * p.a.HKV * p.tiles * 4), 2 * D, 0, st>>>(p);
   return SRSWA_OK;
 }
 template <typename T, int KV>
@@ -441,7 +501,7 @@ extern "C" int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws,
     return SRSWA_WORKSPACE;
   }
   p.part = reinterpret_cast<float*>(ws);
-  const int64_t grid = ((int64_t)p.groups + kXcds - 1) / kXcds * kXcds * p.tiles;
+  const int64_t grid = (p.by_group ? ((int64_t)p.groups + kXcds - 1) / kXcds * kXcds : (int64_t)p.groups) * p.tiles;
   if (grid > 0x7fffffff || (int64_t)a->R * a->HKV * p.nsplit > 0x7fffffff) {
     set_error("%s: grid too large", what);
     return SRSWA_UNSUPPORTED;
