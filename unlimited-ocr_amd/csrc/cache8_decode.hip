@@ -165,7 +165,10 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
   }
   const int pr = n < t.nrows ? t.p0 + tok : -1;        // this lane's row position
   const int end = min(t.pmax + 1, t.kend);
-  const int wlo = a.window > 0 ? t.pmin - a.window : INT_MIN;   // every row's window starts past wlo
+  const int wlo = a.window > 0 ? t.pmin - a.window + 1 : 0;    // first key of the first row's window
+  // the keys this lane's row sees: [my_lo, my_lo + my_span) and [0, my_first)
+  const int my_hi = min(pr, t.kend - 1), my_lo = a.window > 0 ? max(pr - a.window + 1, 0) : 0;
+  const uint32_t my_span = (uint32_t)max(my_hi - my_lo + 1, 0), my_first = (uint32_t)max(min(a.sinks, my_hi + 1), 0);
   const int32_t* topk = nullptr;
   const float* bias = nullptr;
   if constexpr (SEL) {
@@ -290,14 +293,15 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int k = key + 4 * g + j;
-            bool see = key >= 0 && k <= pr && k < t.kend, any = key >= 0 && k < end;
-            if constexpr (SEL) {
-              see = see && k >= lo && k <= hi;
-              any = any && k >= lo && k <= hi;
-            } else if (a.window > 0) {
-              see = see && (k > pr - a.window || k < a.sinks);
-              any = any && (k > wlo || k < a.sinks);
+            bool see, any;
+            if constexpr (SEL) {                           // the tile's rows share one position
+              see = any = (k >= lo) & (k <= hi) & (k < end);
+            } else {
+              see = ((uint32_t)(k - my_lo) < my_span) | ((uint32_t)k < my_first);
+              any = (k < end) & ((k >= wlo) | (k < a.sinks));
             }
+            see = see & (key >= 0);
+            any = any & (key >= 0);
             z[4 * e + j] = see ? z[4 * e + j] : -INFINITY;
             if constexpr (DV == 8) {
               b.v[4 * e + j].x = any ? b.v[4 * e + j].x : 0u;

@@ -77,6 +77,13 @@ __device__ __forceinline__ Tile tile_of(const PrefillK& p, int r, int tile) {
   return t;
 }
 
+// lane q's value, uniform
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int q) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, q);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), q);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // c + the sum of a packed fp16 pair
 __device__ __forceinline__ float dot2_ones(uint32_t w, float c) {
   const f16x2_native_t one = {(_Float16)1.f, (_Float16)1.f};
@@ -132,6 +139,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + 16 * s);
   }
   const int pr = wrow < t.nrows ? t.p0 + tok : -1;
+  // the keys this row sees: [my_lo, my_lo + my_span) and [0, my_first)
+  const int my_hi = min(pr, t.kend - 1), my_lo = a.window > 0 ? max(pr - a.window + 1, 0) : 0;
+  const uint32_t my_span = (uint32_t)max(my_hi - my_lo + 1, 0), my_first = (uint32_t)max(min(a.sinks, my_hi + 1), 0);
   const bool wave_live = wave * 32 < t.nrows;
   const int wpmin = t.p0 + (t.row0 + min(wave * 32, t.nrows - 1)) / p.G;
   const int wpmax = t.p0 + (t.row0 + min(wave * 32 + 31, t.nrows - 1)) / p.G;
@@ -146,68 +156,62 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int wgrp = wave * kWave / PPR / kGroup;                     // the wave's group in pass 0
   const uint32_t koff = (uint32_t)(srow - wgrp * kGroup) * (uint32_t)a.k_st + scol;
   const uint32_t voff = (uint32_t)(srow - wgrp * kGroup) * (uint32_t)a.v_st + scol;
-  typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
-  const scalar_ints bt = (scalar_ints)(a.block_table + (int64_t)r * a.bt_sr);
+  // ONE: read through the scalar cache (constant address space)
+  using Table = std::conditional_t<ONE, const __attribute__((address_space(4))) int32_t*, const int32_t*>;
+  const Table bt = (Table)(a.block_table + (int64_t)r * a.bt_sr);
   const uint8_t* kcache = reinterpret_cast<const uint8_t*>(a.k_cache) + (int64_t)h * a.k_sh;
   const uint8_t* vcache = reinterpret_cast<const uint8_t*>(a.v_cache) + (int64_t)h * a.v_sh;
   const float *kscale = a.k_scale + (int64_t)h * a.ks_sh, *vscale = a.v_scale + (int64_t)h * a.vs_sh;
   auto base_of = [&](int u) { return (u < t.c0 ? u : t.c1 + u - t.c0) * kChunk; };
   auto block_of = [&](int key) { return (int)(__umulhi((uint32_t)key, p.page_mul) >> p.page_shift); };
-  // ONE: pages of a multiple of 64 keys hold whole chunks, one lookup each (the
-  // scalar address arithmetic of four took as long as the conversions: 2,048 rows
-  // after 30,720 keys 555 -> 470 us); else one lookup per 16-key group
-  constexpr int NG = ONE ? 1 : 4;
-  auto of_lane = [&](const int (&v)[NG]) {
-    if constexpr (ONE) return v[0];
-    else return tid & 2 ? (tid & 1 ? v[3] : v[2]) : (tid & 1 ? v[1] : v[0]);
-  };
-  auto of_piece = [&](const int (&v)[NG], int i) {                  // the entry of piece i's group
-    if constexpr (ONE) return v[0];
-    else return D == 128 ? v[i] : (wgrp ? v[1 + 2 * i] : v[2 * i]);
-  };
+  // ONE: pages of a multiple of 64 keys hold whole chunks, whose page and address
+  // are scalar (one 64-bit product each: as scalar arithmetic for four groups this
+  // took as long as the conversions).  Else lane q of each four finds 16-key group
+  // q's, and readlane hands it to the wave.
   auto offset = [](int n, int64_t stride) { return (uint64_t)(uint32_t)n * (uint32_t)stride; };   // (strides below 2^31)
-  int pgn[NG], pgs[NG];              // page ids of the groups: of the chunk to fetch, of the chunk to stage
+  const int lq = ONE ? 0 : tid & 3;
+  int pgn, pgs = 0;                  // page id (of group lq): of the chunk to fetch, of the chunk to stage
   uint2 kb[NP], vb[NP];
-  float gk, gv;                      // the scales of group tid % 4
+  float gk, gv;                      // the page's scales
   auto lookup = [&](int u) __attribute__((always_inline)) {
-    const int j = base_of(min(u, u_hi - 1));
-#pragma unroll
-    for (int q = 0; q < NG; ++q) pgn[q] = bt[block_of(min(j + q * kGroup, t.end - 1))];
+    pgn = bt[block_of(min(base_of(min(u, u_hi - 1)) + lq * kGroup, t.end - 1))];
   };
   auto fetch = [&](int u) __attribute__((always_inline)) {
     const int j = base_of(min(u, u_hi - 1));
-    int safe[NG];
-#pragma unroll
-    for (int q = 0; q < NG; ++q) {
-      pgs[q] = pgn[q];
-      safe[q] = pgn[q] >= 0 && pgn[q] < a.num_pages ? pgn[q] : 0;
-    }
-    const int gp = of_lane(safe);
-    gk = kscale[offset(gp, a.ks_sp)];
-    gv = vscale[offset(gp, a.vs_sp)];
+    pgs = pgn;
+    const int page = pgn >= 0 && pgn < a.num_pages ? pgn : 0;
+    gk = kscale[offset(page, a.ks_sp)];
+    gv = vscale[offset(page, a.vs_sp)];
+    const int key = ONE ? j : min(j + lq * kGroup, t.end - 1) & ~(kGroup - 1);
+    const int rw = key - block_of(key) * a.page_size;
+    const uint64_t ko = offset(page, a.k_sp) + offset(rw, a.k_st), vo = offset(page, a.v_sp) + offset(rw, a.v_st);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int q = D == 128 ? i : wgrp + 2 * i;                    // RPP is 16 or 32 rows
-      const int key = ONE ? j : min(j + q * kGroup, t.end - 1) & ~(kGroup - 1);
-      const int page = of_piece(safe, i), rw = key - block_of(key) * a.page_size + (ONE ? q * kGroup : 0);
-      kb[i] = *reinterpret_cast<const uint2*>(kcache + (offset(page, a.k_sp) + offset(rw, a.k_st)) + koff);
-      vb[i] = *reinterpret_cast<const uint2*>(vcache + (offset(page, a.v_sp) + offset(rw, a.v_st)) + voff);
+      const int q = D == 128 ? i : wgrp + 2 * i;                    // the piece's group: RPP is 16 or 32 rows
+      const uint8_t *kp, *vp;
+      if constexpr (ONE) {
+        kp = kcache + (ko + offset(q * kGroup, a.k_st));
+        vp = vcache + (vo + offset(q * kGroup, a.v_st));
+      } else {
+        kp = kcache + lane_u64(ko, q);
+        vp = vcache + lane_u64(vo, q);
+      }
+      kb[i] = *reinterpret_cast<const uint2*>(kp + koff);
+      vb[i] = *reinterpret_cast<const uint2*>(vp + voff);
     }
   };
   auto stage = [&](int u, int buf) __attribute__((always_inline)) {
     const int j = base_of(u);
-    int ok[NG];
-    bool inside = j + kChunk <= t.end && (a.window == 0 || j > t.pmin - a.window || j + kChunk <= a.sinks);
-#pragma unroll
-    for (int q = 0; q < NG; ++q) {
-      ok[q] = pgs[q] >= 0 && pgs[q] < a.num_pages && j + q * kGroup < t.end;
-      inside = inside && ok[q];
-    }
+    const bool ok = pgs >= 0 && pgs < a.num_pages && j + lq * kGroup < t.end;
+    const uint32_t oks = ONE ? (ok ? 15u : 0u) : (uint32_t)__ballot(ok) & 15u;
+    const bool inside = oks == 15u && j + kChunk <= t.end &&
+                        (a.window == 0 || j > t.pmin - a.window || j + kChunk <= a.sinks);
     if (per_lane(!inside)) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int key = j + srow + i * RPP;
-        const bool any = of_piece(ok, i) && key < t.end && (a.window == 0 || key > t.pmin - a.window || key < a.sinks);
+        const bool any = (oks >> (D == 128 ? i : wgrp + 2 * i) & 1u) && key < t.end &&
+                         (a.window == 0 || key > t.pmin - a.window || key < a.sinks);
         kb[i].x = any ? kb[i].x : 0u;
         kb[i].y = any ? kb[i].y : 0u;
         vb[i].x = any ? vb[i].x : 0u;
@@ -224,10 +228,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       *reinterpret_cast<uint4*>(sV + i * RPP * VP) = make_uint4(v0.x, v0.y, v1.x, v1.y);
     }
     if (tid < 4) {
-      const bool good = of_lane(ok) != 0;
-      const float vs = good ? fmaxf(gv, kScaleMin) : 1.f;
+      const float vs = ok ? fmaxf(gv, kScaleMin) : 1.f;
       reinterpret_cast<float4*>(smem + buf * L::buf + L::kBytes + L::vBytes)[tid] =
-          make_float4(good ? gk * p.scale_l2 : 0.f, __log2f(vs), __builtin_amdgcn_rcpf(vs), good ? 1.f : 0.f);
+          make_float4(ok ? gk * p.scale_l2 : 0.f, ok ? __log2f(vs) : -INFINITY, __builtin_amdgcn_rcpf(vs), 0.f);
     }
   };
 
@@ -261,9 +264,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       float4 gs[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) gs[q] = sg[q];
+      // (a group without a page has K zero and an exponent of -inf, and needs no mask)
       const bool whole = j0 + kChunk - 1 <= wpmin && j0 + kChunk <= t.kend &&
-                         (a.window == 0 || j0 > wpmax - a.window || j0 + kChunk <= a.sinks) &&
-                         gs[0].w * gs[1].w * gs[2].w * gs[3].w != 0.f;
+                         (a.window == 0 || j0 > wpmax - a.window || j0 + kChunk <= a.sinks);
       f32x16_t s[2];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -283,9 +286,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
-            const int k = j0 + 32 * kt + d_row(x, hh);
-            bool see = k <= pr && k < t.kend && gs[2 * kt + x / 8].w != 0.f;
-            if (a.window > 0) see = see && (k > pr - a.window || k < a.sinks);
+            const int k = j0 + 4 * hh + 32 * kt + 8 * (x / 4) + x % 4;
+            const bool see = ((uint32_t)(k - my_lo) < my_span) | ((uint32_t)k < my_first);
             s[kt][x] = see ? s[kt][x] : -INFINITY;
           }
       }
