@@ -4,7 +4,7 @@
 // One workgroup = (request, kv head, tile of 128 rows, part of its keys): four
 // waves of 32 rows, a row being a (token, query head of the group) pair, two
 // workgroups per CU.  Per chunk of 64 keys:
-//   * the chunk's bytes, fetched into registers two chunks ahead, are converted
+//   * the chunk's bytes, fetched into registers three chunks ahead, are converted
 //     once for all four waves and stored to LDS, K in q's type and V in fp16
 //     (both exact), into the buffer that the previous chunk does not use: one
 //     barrier per chunk;
@@ -90,6 +90,36 @@ __device__ __forceinline__ float dot2_ones(uint32_t w, float c) {
   return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_native_t, w), one, c, false);
 }
 
+// Tile number b over all requests' own tiles: its request and place there, the
+// same on every lane; false past the last.
+__device__ __forceinline__ bool nth_tile(const PrefillK& p, int b, int lane, int* r, int* tile) {
+  const srswa_cache8_attend_args& a = p.a;
+  int before = 0;
+  for (int r0 = 0; r0 < a.R; r0 += kWave) {
+    int n = 0;
+    if (r0 + lane < a.R) {
+      const int q0 = min(max(a.cu_seqlens_q[r0 + lane], 0), a.total_q);
+      const int q1 = min(max(a.cu_seqlens_q[r0 + lane + 1], q0), a.total_q);
+      n = (int)(((int64_t)min(q1 - q0, a.max_query_len) * p.G + kRowsWg - 1) / kRowsWg);
+    }
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int x = __shfl_up(incl, o, kWave);
+      if (lane >= o) incl += x;
+    }
+    const uint64_t past = __ballot(before + incl > b);
+    if (past) {
+      const int i = __ffsll((long long)past) - 1;
+      *r = __builtin_amdgcn_readfirstlane(r0 + i);
+      *tile = __builtin_amdgcn_readfirstlane(b - before - __shfl(incl - n, i, kWave));
+      return true;
+    }
+    before += __shfl(incl, kWave - 1, kWave);
+  }
+  return false;
+}
+
 // Parts of a tile: at least eight chunks each.
 __device__ __forceinline__ int parts_of(const PrefillK& p, const Tile& t) {
   return max(1, min(p.nsplit, t.chunks / 8));
@@ -109,20 +139,24 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int rl = lane & 31, hh = lane >> 5;
 
   // The hardware deals workgroups to the XCDs in turn.  One request: the tiles of
-  // one (head, part), which read the same keys, stay on one XCD's L2.  Several: their
-  // lengths are known on the device only, so consecutive workgroups take one tile
-  // of each (request, head, part), which spreads every length over the XCDs.
-  // Later, longer tiles come first.
-  int gi, tile;
+  // one (head, part), which read the same keys, stay on one XCD's L2, the later,
+  // longer ones first.  Several: workgroups count only the tiles that the requests
+  // have, so every XCD gets as many to one (six requests of 70 to 1,900 rows, ten
+  // heads, 500 tiles for 512 places: 81 -> 58 us against tiles up to the longest).
+  int r, tile, h, part;
   if (p.by_group) {
-    gi = (int)(blockIdx.x % kXcds) + kXcds * (int)(blockIdx.x / kXcds / p.tiles);
+    const int gi = (int)(blockIdx.x % kXcds) + kXcds * (int)(blockIdx.x / kXcds / p.tiles);
     if (gi >= p.groups) return;
     tile = p.tiles - 1 - (int)(blockIdx.x / kXcds % p.tiles);
+    part = gi % p.nsplit;
+    h = gi / p.nsplit;
+    r = 0;
   } else {
-    gi = (int)(blockIdx.x % p.groups);
-    tile = p.tiles - 1 - (int)(blockIdx.x / p.groups);
+    const int b = (int)blockIdx.x / p.nsplit;
+    part = (int)blockIdx.x % p.nsplit;
+    h = b % a.HKV;
+    if (!nth_tile(p, b / a.HKV, lane, &r, &tile)) return;
   }
-  const int part = gi % p.nsplit, h = gi / p.nsplit % a.HKV, r = gi / p.nsplit / a.HKV;
   const Tile t = tile_of(p, r, tile);
   if (t.nrows == 0) return;
   const int parts = parts_of(p, t);
@@ -170,18 +204,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   // q's, and readlane hands it to the wave.
   auto offset = [](int n, int64_t stride) { return (uint64_t)(uint32_t)n * (uint32_t)stride; };   // (strides below 2^31)
   const int lq = ONE ? 0 : tid & 3;
-  int pgn, pgs = 0;                  // page id (of group lq): of the chunk to fetch, of the chunk to stage
-  uint2 kb[NP], vb[NP];
-  float gk, gv;                      // the page's scales
+  int pgn;                           // page id (of group lq) of the chunk to fetch next
+  struct Fetched {                   // a chunk's bytes, its page id and scales
+    uint2 kb[NP], vb[NP];
+    float gk, gv;
+    int page;
+  };
+  Fetched fa, fb;                    // of the odd and the even chunks to come
   auto lookup = [&](int u) __attribute__((always_inline)) {
     pgn = bt[block_of(min(base_of(min(u, u_hi - 1)) + lq * kGroup, t.end - 1))];
   };
-  auto fetch = [&](int u) __attribute__((always_inline)) {
+  auto fetch = [&](int u, Fetched& f) __attribute__((always_inline)) {
     const int j = base_of(min(u, u_hi - 1));
-    pgs = pgn;
+    f.page = pgn;
     const int page = pgn >= 0 && pgn < a.num_pages ? pgn : 0;
-    gk = kscale[offset(page, a.ks_sp)];
-    gv = vscale[offset(page, a.vs_sp)];
+    f.gk = kscale[offset(page, a.ks_sp)];
+    f.gv = vscale[offset(page, a.vs_sp)];
     const int key = ONE ? j : min(j + lq * kGroup, t.end - 1) & ~(kGroup - 1);
     const int rw = key - block_of(key) * a.page_size;
     const uint64_t ko = offset(page, a.k_sp) + offset(rw, a.k_st), vo = offset(page, a.v_sp) + offset(rw, a.v_st);
@@ -196,13 +234,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         kp = kcache + lane_u64(ko, q);
         vp = vcache + lane_u64(vo, q);
       }
-      kb[i] = *reinterpret_cast<const uint2*>(kp + koff);
-      vb[i] = *reinterpret_cast<const uint2*>(vp + voff);
+      f.kb[i] = *reinterpret_cast<const uint2*>(kp + koff);
+      f.vb[i] = *reinterpret_cast<const uint2*>(vp + voff);
     }
   };
-  auto stage = [&](int u, int buf) __attribute__((always_inline)) {
+  auto stage = [&](int u, int buf, Fetched& f) __attribute__((always_inline)) {
     const int j = base_of(u);
-    const bool ok = pgs >= 0 && pgs < a.num_pages && j + lq * kGroup < t.end;
+    const bool ok = f.page >= 0 && f.page < a.num_pages && j + lq * kGroup < t.end;
     const uint32_t oks = ONE ? (ok ? 15u : 0u) : (uint32_t)__ballot(ok) & 15u;
     const bool inside = oks == 15u && j + kChunk <= t.end &&
                         (a.window == 0 || j > t.pmin - a.window || j + kChunk <= a.sinks);
@@ -212,25 +250,25 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         const int key = j + srow + i * RPP;
         const bool any = (oks >> (D == 128 ? i : wgrp + 2 * i) & 1u) && key < t.end &&
                          (a.window == 0 || key > t.pmin - a.window || key < a.sinks);
-        kb[i].x = any ? kb[i].x : 0u;
-        kb[i].y = any ? kb[i].y : 0u;
-        vb[i].x = any ? vb[i].x : 0u;
-        vb[i].y = any ? vb[i].y : 0u;
+        f.kb[i].x = any ? f.kb[i].x : 0u;
+        f.kb[i].y = any ? f.kb[i].y : 0u;
+        f.vb[i].x = any ? f.vb[i].x : 0u;
+        f.vb[i].y = any ? f.vb[i].y : 0u;
       }
     }
     uint16_t* sK = reinterpret_cast<uint16_t*>(smem + buf * L::buf) + srow * KP + scol;
     uint16_t* sV = reinterpret_cast<uint16_t*>(smem + buf * L::buf + L::kBytes) + srow * VP + scol;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const uint2 k0 = bytes4_to<KV, T>(kb[i].x), k1 = bytes4_to<KV, T>(kb[i].y);
+      const uint2 k0 = bytes4_to<KV, T>(f.kb[i].x), k1 = bytes4_to<KV, T>(f.kb[i].y);
       *reinterpret_cast<uint4*>(sK + i * RPP * KP) = make_uint4(k0.x, k0.y, k1.x, k1.y);
-      const uint2 v0 = bytes4_to<KV, __half>(vb[i].x), v1 = bytes4_to<KV, __half>(vb[i].y);
+      const uint2 v0 = bytes4_to<KV, __half>(f.vb[i].x), v1 = bytes4_to<KV, __half>(f.vb[i].y);
       *reinterpret_cast<uint4*>(sV + i * RPP * VP) = make_uint4(v0.x, v0.y, v1.x, v1.y);
     }
     if (tid < 4) {
-      const float vs = ok ? fmaxf(gv, kScaleMin) : 1.f;
+      const float vs = ok ? fmaxf(f.gv, kScaleMin) : 1.f;
       reinterpret_cast<float4*>(smem + buf * L::buf + L::kBytes + L::vBytes)[tid] =
-          make_float4(ok ? gk * p.scale_l2 : 0.f, ok ? __log2f(vs) : -INFINITY, __builtin_amdgcn_rcpf(vs), 0.f);
+          make_float4(ok ? f.gk * p.scale_l2 : 0.f, ok ? __log2f(vs) : -INFINITY, __builtin_amdgcn_rcpf(vs), 0.f);
     }
   };
 
@@ -241,19 +279,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 
   if (u_lo < u_hi) {
     lookup(u_lo);
-    fetch(u_lo);
+    fetch(u_lo, fb);
     lookup(u_lo + 1);
-    stage(u_lo, 0);
-    fetch(u_lo + 1);
+    fetch(u_lo + 1, fa);
     lookup(u_lo + 2);
+    stage(u_lo, 0, fb);
+    fetch(u_lo + 2, fb);
+    lookup(u_lo + 3);
   }
   settle(qf);
   __syncthreads();
-  for (int u = u_lo; u < u_hi; ++u) {
-    const int buf = (u - u_lo) & 1;
-    stage(min(u + 1, u_hi - 1), buf ^ 1);
-    fetch(u + 2);
-    lookup(u + 3);
+  // one chunk: the next one (in f) goes to the other buffer, f takes the third next
+  auto step = [&](int u, int buf, Fetched& f) __attribute__((always_inline)) {
+    stage(min(u + 1, u_hi - 1), buf ^ 1, f);
+    fetch(u + 3, f);
+    lookup(u + 4);
     const uint16_t* sK = reinterpret_cast<const uint16_t*>(smem + buf * L::buf);
     const uint16_t* sV = reinterpret_cast<const uint16_t*>(smem + buf * L::buf + L::kBytes);
     const float4* sg = reinterpret_cast<const float4*>(smem + buf * L::buf + L::kBytes + L::vBytes);
@@ -261,9 +301,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     // wave-uniform: does some row see a key, does every row see every key
     const bool some = wave_live && j0 <= wpmax && (a.window == 0 || j0 + kChunk - 1 > wpmin - a.window || j0 < a.sinks);
     if (some) {
-      float4 gs[4];
+      float4 gs[4];                                 // (ONE: four times the same)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) gs[q] = sg[q];
+      for (int q = 0; q < 4; ++q) gs[q] = sg[ONE ? 0 : q];
       // (a group without a page has K zero and an exponent of -inf, and needs no mask)
       const bool whole = j0 + kChunk - 1 <= wpmin && j0 + kChunk <= t.kend &&
                          (a.window == 0 || j0 > wpmax - a.window || j0 + kChunk <= a.sinks);
@@ -330,6 +370,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         }
     }
     __syncthreads();
+  };
+  for (int u = u_lo; u < u_hi; u += 2) {
+    step(u, 0, fa);
+    if (u + 1 < u_hi) step(u + 1, 1, fb);
   }
 
   l = xor32_sum(l);
@@ -424,19 +468,22 @@ PrefillK plan(const srswa_cache8_attend_args* a) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, keys / kChunk / 8));
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
-  const int64_t slots = std::max(1, cus / kXcds * 2);
+  p.by_group = a->R == 1;
+  // places for workgroups, and the workgroups of one part: an XCD's share of one
+  // request's, or all of several requests' (half a tile per request is a remainder)
+  const int64_t slots = p.by_group ? std::max(1, cus / kXcds * 2) : 2 * cus;
+  const int64_t all = std::max<int64_t>(1, ((int64_t)a->total_q * p.G / kRowsWg + a->R / 2) * a->HKV);
   double best = 1e30;
   p.nsplit = 1;
   for (int n = 1; n <= most; ++n) {
-    const int64_t per_xcd = ((int64_t)a->R * a->HKV * n + kXcds - 1) / kXcds * p.tiles;
-    const double cost = (double)((per_xcd + slots - 1) / slots) / n;
+    const int64_t wgs = p.by_group ? ((int64_t)a->HKV * n + kXcds - 1) / kXcds * p.tiles : all * n;
+    const double cost = (double)((wgs + slots - 1) / slots) / n;
     if (cost < best * 0.95) {
       best = cost;
       p.nsplit = n;
     }
   }
   p.groups = a->R * a->HKV * p.nsplit;
-  p.by_group = a->R == 1;
   return p;
 }
 
@@ -503,7 +550,9 @@ extern "C" int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws,
     return SRSWA_WORKSPACE;
   }
   p.part = reinterpret_cast<float*>(ws);
-  const int64_t grid = (p.by_group ? ((int64_t)p.groups + kXcds - 1) / kXcds * kXcds : (int64_t)p.groups) * p.tiles;
+  // several requests: as many tiles as their rows can make
+  const int64_t own = std::min<int64_t>((int64_t)a->R * p.tiles, (int64_t)a->total_q * p.G / kRowsWg + a->R);
+  const int64_t grid = p.by_group ? ((int64_t)p.groups + kXcds - 1) / kXcds * kXcds * p.tiles : own * a->HKV * p.nsplit;
   if (grid > 0x7fffffff || (int64_t)a->R * a->HKV * p.nsplit > 0x7fffffff) {
     set_error("%s: grid too large", what);
     return SRSWA_UNSUPPORTED;
