@@ -211,8 +211,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     int page;
   };
   Fetched fa, fb;                    // of the odd and the even chunks to come
-  auto lookup = [&](int u) __attribute__((always_inline)) {
-    pgn = bt[block_of(min(base_of(min(u, u_hi - 1)) + lq * kGroup, t.end - 1))];
+  auto page_of = [&](int u) __attribute__((always_inline)) {
+    return bt[block_of(min(base_of(min(u, u_hi - 1)) + lq * kGroup, t.end - 1))];
   };
   auto fetch = [&](int u, Fetched& f) __attribute__((always_inline)) {
     const int j = base_of(min(u, u_hi - 1));
@@ -278,14 +278,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   float m = -INFINITY, msub = 0.f, thr = -INFINITY, l = 0.f;
 
   if (u_lo < u_hi) {
-    lookup(u_lo);
+    // the pages of the first chunks at once: loads return in order
+    const int p0 = page_of(u_lo), p1 = page_of(u_lo + 1), p2 = page_of(u_lo + 2), p3 = page_of(u_lo + 3);
+    pgn = p0;
     fetch(u_lo, fb);
-    lookup(u_lo + 1);
+    pgn = p1;
     fetch(u_lo + 1, fa);
-    lookup(u_lo + 2);
     stage(u_lo, 0, fb);
+    pgn = p2;
     fetch(u_lo + 2, fb);
-    lookup(u_lo + 3);
+    pgn = p3;
   }
   settle(qf);
   __syncthreads();
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   auto step = [&](int u, int buf, Fetched& f) __attribute__((always_inline)) {
     stage(min(u + 1, u_hi - 1), buf ^ 1, f);
     fetch(u + 3, f);
-    lookup(u + 4);
+    pgn = page_of(u + 4);
     const uint16_t* sK = reinterpret_cast<const uint16_t*>(smem + buf * L::buf);
     const uint16_t* sV = reinterpret_cast<const uint16_t*>(smem + buf * L::buf + L::kBytes);
     const float4* sg = reinterpret_cast<const float4*>(smem + buf * L::buf + L::kBytes + L::vBytes);
@@ -468,21 +470,23 @@ PrefillK plan(const srswa_cache8_attend_args* a) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, keys / kChunk / 8));
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
-  p.by_group = a->R == 1;
-  // places for workgroups, and the workgroups of one part: an XCD's share of one
-  // request's, or all of several requests' (half a tile per request is a remainder)
-  const int64_t slots = p.by_group ? std::max(1, cus / kXcds * 2) : 2 * cus;
-  const int64_t all = std::max<int64_t>(1, ((int64_t)a->total_q * p.G / kRowsWg + a->R / 2) * a->HKV);
-  double best = 1e30;
-  p.nsplit = 1;
-  for (int n = 1; n <= most; ++n) {
-    const int64_t wgs = p.by_group ? ((int64_t)a->HKV * n + kXcds - 1) / kXcds * p.tiles : all * n;
-    const double cost = (double)((wgs + slots - 1) / slots) / n;
-    if (cost < best * 0.95) {
-      best = cost;
-      p.nsplit = n;
+  // rounds of the GPU per part, tiles dealt in turn (half a tile per request is a
+  // remainder) or one request's by XCD, and the parts that need the least
+  const int64_t in_turn = std::max<int64_t>(1, ((int64_t)a->total_q * p.G / kRowsWg + a->R / 2) * a->HKV);
+  double least[2] = {1e30, 1e30};
+  int parts[2] = {1, 1};
+  for (int g = 0; g < (a->R == 1 ? 2 : 1); ++g)
+    for (int n = 1; n <= most; ++n) {
+      const int64_t wgs = g ? ((int64_t)a->HKV * n + kXcds - 1) / kXcds * p.tiles : in_turn * n;
+      const int64_t slots = g ? std::max(1, cus / kXcds * 2) : 2 * cus;
+      const double cost = (double)((wgs + slots - 1) / slots) / n;
+      if (cost < least[g] * 0.95) {
+        least[g] = cost;
+        parts[g] = n;
+      }
     }
-  }
+  p.by_group = least[1] <= least[0] * 1.02;
+  p.nsplit = parts[p.by_group];
   p.groups = a->R * a->HKV * p.nsplit;
   return p;
 }
