@@ -79,6 +79,13 @@ __device__ __forceinline__ void settle(uint4 (&v)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i].x), "+v"(v[i].y), "+v"(v[i].z), "+v"(v[i].w));
 }
 
+// lane q's value, uniform
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int q) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, q);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), q);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // two fp32 values -> packed fp16, round to nearest even (v_cvt_pk_f16_f32)
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const f16x2_native_t v = {(_Float16)lo, (_Float16)hi};

@@ -2,10 +2,13 @@
 // (gfx950): every key, a sliding window with first tokens that stay visible, or
 // selected blocks.
 //
-// One workgroup = (request, kv head, 16-row tile, chunk of keys); its rows are
-// the tile's (token, query head of the group) pairs, so a K/V byte is loaded
-// once for all of them.  Four waves take units of 32 keys in turn, entirely in
-// registers:
+// An item is a 16-row tile of a request: rows are (token, query head of the group)
+// pairs, so a K/V byte is loaded once for all of them.  A workgroup works for one
+// kv head, on one item whole or, where items are long or few, on an equal share of
+// the units (32 keys each) of all items together, which leaves no last round of a
+// ragged batch: it cuts at most its first and its last item, and
+// cache8_merge_kernel joins what was cut.  The waves of a workgroup take an item's
+// units in turn, entirely in registers:
 //   S^T = K Q^T   v_mfma_f32_16x16x32: A = 16 keys x 32 dims.  The reduction
 //         runs over the dims in any order, so a lane takes 16 contiguous bytes
 //         of a key row per load (two steps) and Q's operand follows suit.
@@ -23,7 +26,6 @@
 // (half a step 2^-12; bf16 would lose 2^-9 of each weight).  The running maximum
 // moves only when a z' exceeds it by 2^8 and is kept 2^7 below it, so p' stays
 // below 2^15 and only weights under 2^-31 of the largest vanish.
-// Chunks of one tile are joined by cache8_merge_kernel.
 #include <algorithm>
 
 #include "cache8.h"
@@ -34,24 +36,25 @@ namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
 constexpr int kRows = 16;
 constexpr float kBelow = 7.f, kSlack = 8.f;   // the running maximum's place and play (log2)
 constexpr int kGroup = 16;     // keys per page lookup; a unit is two groups
+constexpr int kMinShare = 16;  // units of the smallest share
 
 struct AttendK {
   srswa_cache8_attend_args a;
   int G;                  // query heads per kv head
-  int tiles, nchunk, upc; // row tiles and chunks per (request, kv head), units per chunk
+  int tiles, items;       // row tiles per request, items in all (R * tiles)
+  int shares;             // workgroups per kv head that share the items' units; 0: one per item
   int rs;                 // rows of a record
   int gpp;                // 16-key groups per page
   float scale_l2;         // scale * log2(e)
-  float* part;            // records: [R * tiles * HKV][nchunk][rs * (D + 2)]
+  float* part;            // records: [shares][HKV][2][rs * (D + 2)], a share's first item and its last
 };
 
 // What a row tile reads, the same on every thread and in the merge kernel.
 struct Tile {
+  int r;                  // request
   int row0, nrows;        // rows of the tile: (token t, head g) = (row / G, row % G)
   int q0;                 // first query token of the request
   int p0;                 // position of the request's first query row
@@ -64,6 +67,7 @@ template <bool SEL>
 __device__ __forceinline__ Tile tile_of(const AttendK& p, int r, int tile) {
   const srswa_cache8_attend_args& a = p.a;
   Tile t;
+  t.r = r;
   const int q0 = a.cu_seqlens_q ? min(max(a.cu_seqlens_q[r], 0), a.total_q) : r * a.max_query_len;
   const int q1 = a.cu_seqlens_q ? min(max(a.cu_seqlens_q[r + 1], q0), a.total_q) : q0 + a.max_query_len;
   const int sl = max(a.seq_lens[r], 0);
@@ -93,6 +97,52 @@ __device__ __forceinline__ Tile tile_of(const AttendK& p, int r, int tile) {
   const int ng1 = SEL && a.window == 0 ? 0 : max((end + kGroup - 1) / kGroup - t.g1, 0);
   t.units = t.nrows > 0 ? (t.ng0 + ng1 + 1) / 2 : 0;
   return t;
+}
+
+// Units that an item counts for: one at least, so that a row without keys is written.
+template <bool SEL>
+__device__ __forceinline__ uint32_t item_units(const AttendK& p, int item) {
+  if (item >= p.items) return 0u;
+  const Tile t = tile_of<SEL>(p, item / p.tiles, item % p.tiles);
+  return t.nrows > 0 ? (uint32_t)max(t.units, 1) : 0u;
+}
+
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v, int lane) {   // inclusive
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint32_t x = __shfl_up(v, o, kWave);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+
+// The units of all items (a wave's 64 items sum below 2^32: a request holds 2^30 keys at most).
+template <bool SEL>
+__device__ __forceinline__ int64_t all_units(const AttendK& p, int lane) {
+  int64_t n = 0;
+  for (int i0 = 0; i0 < p.items; i0 += kWave) n += (uint32_t)wave_sum_int((int)item_units<SEL>(p, i0 + lane));
+  return n;
+}
+__device__ __forceinline__ int share_count(const AttendK& p, int64_t total) {
+  return (int)max((int64_t)1, min((int64_t)p.shares, total / kMinShare));
+}
+
+// The item that holds unit u of all, and the unit it starts at; false past the last.
+template <bool SEL>
+__device__ __forceinline__ bool item_at(const AttendK& p, int64_t u, int lane, int* item, int64_t* start) {
+  int64_t before = 0;
+  for (int i0 = 0; i0 < p.items; i0 += kWave) {
+    const uint32_t n = item_units<SEL>(p, i0 + lane), incl = wave_prefix(n, lane);
+    const uint64_t past = __ballot(before + (int64_t)incl > u);
+    if (past) {
+      const int i = __ffsll((long long)past) - 1;
+      *item = __builtin_amdgcn_readfirstlane(i0 + i);
+      *start = before + (uint32_t)__builtin_amdgcn_readlane((int)(incl - n), i);
+      return true;
+    }
+    before += (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
+  }
+  return false;
 }
 
 // 4 x 4 byte transpose: word t of the result holds byte t of a, b, c, d
@@ -132,27 +182,19 @@ struct UnitBytes {
   std::conditional_t<DV == 8, uint2, uint32_t> v[8];   // keys 4 (l / 16) + 0..3 of each group
 };
 
-template <typename T, int KV, int D, bool SEL>
-__global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
+// Item rows' attention over units [u_lo, u_end) of theirs: to out and lse, or to a
+// record (unnormalised, with m and l) where rec is not null.
+template <typename T, int KV, int D, bool SEL, int NW>
+__device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile& t, int u_lo, int u_end, float* rec) {
+  constexpr int NT = NW * kWave;
   constexpr int NL = D / 64;      // K loads per group
   constexpr int DV = D / 16;      // V tiles
   using VB = std::conditional_t<DV == 8, uint2, uint32_t>;
-  __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
-  __shared__ __align__(16) float s_o[kWaves][kRows][D];
+  __shared__ float s_m[NW][kRows], s_l[NW][kRows];
+  __shared__ __align__(16) float s_o[NW][kRows][D];
   const srswa_cache8_attend_args& a = p.a;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int n = lane & 15, g = lane >> 4;
-
-  // the heads of one chunk run side by side (their rows share DRAM pages); a
-  // tile's later chunks come after every tile's earlier ones
-  int lid = (int)blockIdx.x;
-  const int h = lid % a.HKV;
-  lid /= a.HKV;
-  const int rt = lid % (a.R * p.tiles), chunk = lid / (a.R * p.tiles);
-  const int r = rt / p.tiles;
-  const Tile t = tile_of<SEL>(p, r, rt % p.tiles);
-  if (t.nrows == 0 || (chunk > 0 && chunk * p.upc >= t.units)) return;
-  const int u_end = min(t.units, (chunk + 1) * p.upc);
+  const int n = lane & 15, g = lane >> 4, r = t.r;
 
   // Q operand: lane (row n, g) holds dims 64 i + 16 g + 8 e .. + 7 of step 2 i + e
   const int row = min(t.row0 + n, t.row0 + t.nrows - 1);
@@ -187,13 +229,14 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
   const int64_t koff = (int64_t)n * a.k_st + 16 * g;
   const int64_t voff = (int64_t)(4 * g) * a.v_st + DV * n;
 
-  for (int u0 = chunk * p.upc + wave; u0 < u_end; u0 += kWaves * kWave) {
+  for (int u0 = u_lo + wave; u0 < u_end; u0 += NW * kWave) {
     // lane i looks up the two groups of this wave's i-th unit from here: first
-    // key (-1: nothing to see), page and row in it, scales, bias and bounds
-    int dk[2], dpage[2], drow[2], dlo[2], dhi[2];
+    // key (-1: nothing to see), byte offsets, scales, bias and bounds
+    int dk[2], dlo[2], dhi[2];
+    uint64_t dko[2], dvo[2];
     float dks[2], dvi[2], db[2];
     bool whole = true;
-    const int du = u0 + kWaves * lane;
+    const int du = u0 + NW * lane;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int gi = 2 * du + e;
@@ -227,8 +270,9 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
       if (key >= 0) page = a.block_table[(int64_t)r * a.bt_sr + key / a.page_size];
       const bool ok = page >= 0 && page < a.num_pages;
       dk[e] = ok ? key : -1;
-      dpage[e] = ok ? page : 0;
-      drow[e] = ok ? key % a.page_size : 0;
+      const uint32_t pg = ok ? page : 0, rw = ok ? key % a.page_size : 0;   // (strides are below 2^31)
+      dko[e] = (uint64_t)pg * (uint32_t)a.k_sp + (uint64_t)rw * (uint32_t)a.k_st;
+      dvo[e] = (uint64_t)pg * (uint32_t)a.v_sp + (uint64_t)rw * (uint32_t)a.v_st;
       dks[e] = ok ? p.scale_l2 * a.k_scale[(int64_t)page * a.ks_sp + (int64_t)h * a.ks_sh] : 0.f;
       const float vs = ok ? fmaxf(a.v_scale[(int64_t)page * a.vs_sp + (int64_t)h * a.vs_sh], kScaleMin) : 1.f;
       dvi[e] = 1.f / vs;
@@ -242,25 +286,33 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
     }
     const uint64_t whole_bits = __ballot(whole);
     settle(qf);
-    const int cnt = min(kWave, (u_end - u0 + kWaves - 1) / kWaves);
+    const int cnt = min(kWave, (u_end - u0 + NW - 1) / NW);
 
-    auto load = [&](int i, UnitBytes<D>& b) __attribute__((always_inline)) {
+    // One unit's bytes are held at a time: K's registers are loaded again as soon as
+    // the products have read them, V's after the transposes, so a unit's K comes in
+    // behind the softmax and its V behind the next products, and four waves fit a SIMD
+    UnitBytes<D> b;
+    auto load_k = [&](int i) __attribute__((always_inline)) {
+      i = min(i, cnt - 1);                       // (past the end: the last unit again, not used)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int page = __builtin_amdgcn_readlane(dpage[e], i), rw = __builtin_amdgcn_readlane(drow[e], i);
-        const uint8_t* kp = kcache + (int64_t)page * a.k_sp + (int64_t)rw * a.k_st + koff;
-        const uint8_t* vp = vcache + (int64_t)page * a.v_sp + (int64_t)rw * a.v_st + voff;
+        const uint8_t* kp = kcache + lane_u64(dko[e], i) + koff;
 #pragma unroll
         for (int q = 0; q < NL; ++q) b.k[e][q] = *reinterpret_cast<const uint4*>(kp + 64 * q);
+      }
+    };
+    auto load_v = [&](int i) __attribute__((always_inline)) {
+      i = min(i, cnt - 1);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint8_t* vp = vcache + lane_u64(dvo[e], i) + voff;
 #pragma unroll
         for (int j = 0; j < 4; ++j) b.v[4 * e + j] = *reinterpret_cast<const VB*>(vp + (int64_t)j * a.v_st);
       }
     };
-    UnitBytes<D> nx;
-    load(0, nx);
+    load_k(0);
+    load_v(0);
     for (int i = 0; i < cnt; ++i) {
-      UnitBytes<D> b = nx;
-      if (i + 1 < cnt) load(i + 1, nx);
       // S^T
       f32x4_t sc[2];
 #pragma unroll
@@ -274,6 +326,7 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
           sc[e] = mfma16<T>(make_uint4(k2.x, k2.y, k3.x, k3.y), qf[2 * q + 1], sc[e]);
         }
       }
+      load_k(i + 1);
       float z[8];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -340,6 +393,7 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
       const uint4 pa = make_uint4(pack_f16(pe[0], pe[1]), pack_f16(pe[2], pe[3]), pack_f16(pe[4], pe[5]),
                                   pack_f16(pe[6], pe[7]));
       // O += P V
+      uint32_t tv[DV][2];                        // dim d's 8 keys
 #pragma unroll
       for (int hf = 0; hf < DV / 4; ++hf) {
         uint32_t w[8], ta[4], tb[4];
@@ -352,14 +406,20 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
         transpose4(w[4], w[5], w[6], w[7], tb);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const uint2 x0 = bytes4_to<KV, __half>(ta[d]), x1 = bytes4_to<KV, __half>(tb[d]);
-          acc[4 * hf + d] = mfma16<__half>(pa, make_uint4(x0.x, x0.y, x1.x, x1.y), acc[4 * hf + d]);
+          tv[4 * hf + d][0] = ta[d];
+          tv[4 * hf + d][1] = tb[d];
         }
+      }
+      load_v(i + 1);
+#pragma unroll
+      for (int d = 0; d < DV; ++d) {
+        const uint2 x0 = bytes4_to<KV, __half>(tv[d][0]), x1 = bytes4_to<KV, __half>(tv[d][1]);
+        acc[d] = mfma16<__half>(pa, make_uint4(x0.x, x0.y, x1.x, x1.y), acc[d]);
       }
     }
   }
 
-  // the four waves' (m, l, O) of the tile: O lane layout row 4 g + j, dims DV n + d
+  // the waves' (m, l, O): O lane layout row 4 g + j, dims DV n + d
   l = xor32_sum(xor16_sum(l));
   if (g == 0) {
     s_m[wave][n] = m;
@@ -374,22 +434,20 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
             make_float4(acc[d][j], acc[d + 1][j], acc[d + 2][j], acc[d + 3][j]);
     }
   __syncthreads();
-  const bool only = t.units <= p.upc;
-  float* rec = only ? nullptr : p.part + ((int64_t)(rt * a.HKV + h) * p.nchunk + chunk) * p.rs * (D + 2);
-  for (int i = tid; i < t.nrows * (D / 4); i += kThreads) {
+  for (int i = tid; i < t.nrows * (D / 4); i += NT) {
     const int rr = i / (D / 4), c = i % (D / 4) * 4;
     float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][rr]);
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w][rr]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float f = s_m[w][rr] == -INFINITY ? 0.f : exp2f(s_m[w][rr] - M);
       const float4 x = *reinterpret_cast<const float4*>(&s_o[w][rr][c]);
       L = fmaf(f, s_l[w][rr], L);
       o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
     }
-    if (only) {
+    if (!rec) {
       const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
       const float inv = M == -INFINITY ? 0.f : 1.f / L;
       T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn + (int64_t)ho * a.o_sh + c;
@@ -410,39 +468,107 @@ __global__ __launch_bounds__(kThreads) void cache8_decode_kernel(AttendK p) {
   }
 }
 
-// Joins a tile's chunks: one workgroup per (request, tile, kv head).
-template <typename T, int D, bool SEL>
-__global__ __launch_bounds__(kThreads) void cache8_merge_kernel(AttendK p) {
+// shares == 0: one workgroup per (item, kv head).  Else workgroup (share, kv head)
+// takes its equal part of all items' units.  The heads of one share run side by
+// side, on neighbouring XCDs: their rows share DRAM pages (a share's heads on one
+// XCD 305 us, one head's shares first 340 us against 261 us, 48 requests of 700 to
+// 40,000 keys, ten heads).
+template <typename T, int KV, int D, bool SEL, int NW>
+__global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3))) void cache8_decode_kernel(AttendK p) {
   const srswa_cache8_attend_args& a = p.a;
-  const int h = (int)blockIdx.x % a.HKV, rt = (int)blockIdx.x / a.HKV;
-  const Tile t = tile_of<SEL>(p, rt / p.tiles, rt % p.tiles);
-  if (t.nrows == 0 || t.units <= p.upc) return;
-  const int nc = (t.units + p.upc - 1) / p.upc;
-  const int64_t rsz = (int64_t)p.rs * (D + 2);
-  const float* rec = p.part + (int64_t)(rt * a.HKV + h) * p.nchunk * rsz;
-  for (int i = threadIdx.x; i < t.nrows * (D / 4); i += kThreads) {
-    const int rr = i / (D / 4), c = i % (D / 4) * 4;
-    float M = -INFINITY, L = 0.f;
-    for (int k = 0; k < nc; ++k) M = fmaxf(M, rec[k * rsz + p.rs * D + rr]);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < nc; ++k) {
-      const float mk = rec[k * rsz + p.rs * D + rr];
-      const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
-      const float4 x = *reinterpret_cast<const float4*>(rec + k * rsz + rr * D + c);
-      L = fmaf(f, rec[k * rsz + p.rs * D + p.rs + rr], L);
-      o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
-    }
-    const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
-    const float inv = M == -INFINITY ? 0.f : 1.f / L;
-    uint2 w;
-    w.x = Mfma<T>::pack2(o.x * inv, o.y * inv);
-    w.y = Mfma<T>::pack2(o.z * inv, o.w * inv);
-    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn +
-                              (int64_t)ho * a.o_sh + c) = w;
-    if (a.lse && c == 0)
-      a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] =
-          M == -INFINITY ? -INFINITY : (M + log2f(L)) * kLn2;
+  const int lane = threadIdx.x % kWave;
+  const int h = (int)blockIdx.x % a.HKV, id = (int)blockIdx.x / a.HKV;
+  if (p.shares == 0) {
+    const Tile t = tile_of<SEL>(p, id / p.tiles, id % p.tiles);
+    if (t.nrows > 0) attend_item<T, KV, D, SEL, NW>(p, h, t, 0, t.units, nullptr);
+    return;
   }
+  const int64_t total = all_units<SEL>(p, lane);
+  const int n = share_count(p, total);
+  if (id >= n) return;
+  int64_t s = total * id / n;
+  const int64_t e = total * (id + 1) / n;
+  int item;
+  int64_t start;
+  if (!item_at<SEL>(p, s, lane, &item, &start)) return;
+  float* recs = p.part + ((int64_t)id * a.HKV + h) * 2 * p.rs * (D + 2);
+  for (bool first = true; s < e; ++item) {
+    const Tile t = tile_of<SEL>(p, item / p.tiles, item % p.tiles);
+    if (t.nrows == 0) continue;
+    const int64_t end = start + max(t.units, 1);
+    const bool whole = s == start && e >= end;
+    if (!first) __syncthreads();                 // the item before is written from LDS
+    attend_item<T, KV, D, SEL, NW>(p, h, t, (int)(s - start), (int)min((int64_t)t.units, min(e, end) - start),
+                                   whole ? nullptr : recs + (first ? 0 : p.rs * (D + 2)));
+    first = false;
+    s = start = end;
+  }
+}
+
+// Joins the shares of an item that was cut: one wave per (item, kv head, row), D / 64
+// dims a lane.  Share i begins with the item (its first record) unless the item
+// starts inside it (its last).
+template <typename T, int D, bool SEL>
+__global__ __launch_bounds__(kWave) void cache8_merge_kernel(AttendK p) {
+  constexpr int DL = D / kWave;
+  const srswa_cache8_attend_args& a = p.a;
+  const int lane = threadIdx.x;
+  const int rr = (int)blockIdx.x % p.rs, h = (int)blockIdx.x / p.rs % a.HKV, item = (int)blockIdx.x / p.rs / a.HKV;
+  const Tile t = tile_of<SEL>(p, item / p.tiles, item % p.tiles);
+  if (rr >= t.nrows) return;
+  int64_t start = 0, total = 0;
+  for (int i0 = 0; i0 < p.items; i0 += kWave) {
+    const int n = (int)item_units<SEL>(p, i0 + lane);
+    total += (uint32_t)wave_sum_int(n);
+    start += (uint32_t)wave_sum_int(i0 + lane < item ? n : 0);
+  }
+  const int64_t end = start + max(t.units, 1);
+  const int n = share_count(p, total);
+  // the shares that hold units start and end - 1: share i is [total i / n, total (i + 1) / n)
+  auto share_of = [&](int64_t u) {
+    int i = (int)(u * n / total);
+    while (total * (i + 1) / n <= u) ++i;
+    while (total * i / n > u) --i;
+    return i;
+  };
+  const int s0 = share_of(start), s1 = share_of(end - 1);
+  if (s0 == s1) return;                          // not cut
+  const int64_t rsz = (int64_t)p.rs * (D + 2);
+  auto record = [&](int i) {
+    return p.part + (((int64_t)i * a.HKV + h) * 2 + (i == s0 && total * i / n != start ? 1 : 0)) * rsz;
+  };
+  float M = -INFINITY;
+  for (int i = s0 + lane; i <= s1; i += kWave) M = fmaxf(M, record(i)[p.rs * D + rr]);
+  M = wave_max(M);
+  float o[DL] = {}, L = 0.f;
+  for (int i0 = s0; i0 <= s1; i0 += kWave) {
+    const int cnt = min(kWave, s1 - i0 + 1);
+    float f = 0.f, lk = 0.f;                     // lane k: share i0 + k
+    if (lane < cnt) {
+      const float* rec = record(i0 + lane);
+      const float mk = rec[p.rs * D + rr];
+      f = mk == -INFINITY ? 0.f : exp2f(mk - M);
+      lk = f * rec[p.rs * D + p.rs + rr];
+    }
+    L += wave_sum(lk);
+    for (int k = 0; k < cnt; ++k) {
+      const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k));
+      const float* rec = record(i0 + k) + rr * D + DL * lane;
+#pragma unroll
+      for (int d = 0; d < DL; ++d) o[d] = fmaf(fk, rec[d], o[d]);
+    }
+  }
+  const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
+  const float inv = M == -INFINITY ? 0.f : 1.f / L;
+  T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn + (int64_t)ho * a.o_sh + DL * lane;
+  if constexpr (DL == 2) {
+    *reinterpret_cast<uint32_t*>(op) = Mfma<T>::pack2(o[0] * inv, o[1] * inv);
+  } else {
+    *reinterpret_cast<uint16_t*>(op) = (uint16_t)(Mfma<T>::pack2(o[0] * inv, 0.f) & 0xffffu);
+  }
+  if (a.lse && lane == 0)
+    a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] =
+        M == -INFINITY ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -505,8 +631,8 @@ int cache8_check(const srswa_cache8_attend_args* a, const char* what) {
 
 namespace {
 
-// Chunks: enough workgroups to fill the GPU several times, at least 16 units
-// (four per wave) and at most 64 each, so that requests of uneven length spread.
+// Items of at most 64 units (2,048 keys) are taken whole where they make 128
+// workgroups; others are shared by as many workgroups as the GPU holds at once.
 AttendK plan(const srswa_cache8_attend_args* a) {
   AttendK p{};
   p.a = *a;
@@ -515,28 +641,29 @@ AttendK plan(const srswa_cache8_attend_args* a) {
   p.scale_l2 = a->scale * kLog2e;
   const int64_t rows = (int64_t)a->max_query_len * p.G;
   p.tiles = (int)(a->topk ? (int64_t)a->max_query_len * ((p.G + kRows - 1) / kRows) : (rows + kRows - 1) / kRows);
+  p.items = a->R * p.tiles;
   p.rs = (int)std::min<int64_t>(kRows, a->topk ? p.G : rows);
-  const int64_t cap = (int64_t)a->max_blocks * a->page_size;
-  int64_t groups = cap / kGroup;
+  int64_t groups = (int64_t)a->max_blocks * a->page_size / kGroup;
   if (a->topk) groups = (int64_t)a->topk_n * p.gpp + std::min<int64_t>(groups, a->window / kGroup + 2);
   else if (a->window > 0)
     groups = std::min<int64_t>(groups, ((int64_t)a->window + a->max_query_len) / kGroup + 2 + (a->sinks + kGroup - 1) / kGroup);
-  const int64_t units = (groups + 1) / 2;
-  const int64_t w = std::max<int64_t>(1, (int64_t)a->R * a->HKV * p.tiles);
-  p.upc = (int)std::min<int64_t>(64, std::max<int64_t>(16, units * w / 4096));
-  p.nchunk = (int)std::max<int64_t>(1, (units + p.upc - 1) / p.upc);
+  const int64_t units = (groups + 1) / 2, wgs = (int64_t)p.items * a->HKV;
+  int cus = device_cu_count();
+  if (cus <= 0) cus = 256;
+  if (units > 64 || (units > kMinShare && wgs < 128))
+    p.shares = (int)std::min<int64_t>(std::max(1, 3 * cus / a->HKV), (units * p.items + kMinShare - 1) / kMinShare);
   return p;
 }
 
 size_t ws_bytes_of(const AttendK& p) {
-  return p.nchunk > 1 ? (size_t)p.a.R * p.tiles * p.a.HKV * p.nchunk * p.rs * (p.a.D + 2) * sizeof(float) : 0;
+  return (size_t)p.shares * p.a.HKV * 2 * p.rs * (p.a.D + 2) * sizeof(float);
 }
 
 template <typename T, int KV, int D, bool SEL>
 void launch(const AttendK& p, unsigned grid, hipStream_t st) {
-  cache8_decode_kernel<T, KV, D, SEL><<<grid, kThreads, 0, st>>>(p);
-  if (p.nchunk > 1)
-    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.a.R * p.tiles * p.a.HKV), kThreads, 0, st>>>(p);
+  cache8_decode_kernel<T, KV, D, SEL, 4><<<grid, 4 * kWave, 0, st>>>(p);
+  if (p.shares > 0)
+    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.items * p.a.HKV * p.rs), kWave, 0, st>>>(p);
 }
 template <typename T, int KV, int D>
 void launch_sel(const AttendK& p, unsigned grid, hipStream_t st) {
@@ -564,8 +691,8 @@ int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_byt
     return SRSWA_WORKSPACE;
   }
   p.part = reinterpret_cast<float*>(ws);
-  const int64_t grid = (int64_t)a->R * p.tiles * a->HKV * p.nchunk;
-  if (grid > 0x7fffffff) {
+  const int64_t grid = (int64_t)(p.shares > 0 ? p.shares : p.items) * a->HKV;
+  if (grid > 0x7fffffff || (int64_t)a->R * p.tiles * a->HKV * p.rs > 0x7fffffff) {
     set_error("%s: grid too large", what);
     return SRSWA_UNSUPPORTED;
   }

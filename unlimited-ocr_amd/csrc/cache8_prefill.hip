@@ -77,13 +77,6 @@ __device__ __forceinline__ Tile tile_of(const PrefillK& p, int r, int tile) {
   return t;
 }
 
-// lane q's value, uniform
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int q) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, q);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), q);
-  return (uint64_t)hi << 32 | lo;
-}
-
 // c + the sum of a packed fp16 pair
 __device__ __forceinline__ float dot2_ones(uint32_t w, float c) {
   const f16x2_native_t one = {(_Float16)1.f, (_Float16)1.f};
