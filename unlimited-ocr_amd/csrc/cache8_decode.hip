@@ -46,6 +46,7 @@ struct AttendK {
   int G;                  // query heads per kv head
   int tiles, items;       // row tiles per request, items in all (R * tiles)
   int shares;             // workgroups per kv head that share the items' units; 0: one per item
+  bool pairs;             // D = 64: neighbouring heads to one XCD
   int rs;                 // rows of a record
   int gpp;                // 16-key groups per page
   float scale_l2;         // scale * log2(e)
@@ -116,28 +117,35 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v, int lane) {   // inc
   return v;
 }
 
-// The units of all items (a wave's 64 items sum below 2^32: a request holds 2^30 keys at most).
-template <bool SEL>
-__device__ __forceinline__ int64_t all_units(const AttendK& p, int lane) {
-  int64_t n = 0;
-  for (int i0 = 0; i0 < p.items; i0 += kWave) n += (uint32_t)wave_sum_int((int)item_units<SEL>(p, i0 + lane));
-  return n;
-}
+// (a wave's 64 items sum below 2^32: a request holds 2^30 keys at most)
 __device__ __forceinline__ int share_count(const AttendK& p, int64_t total) {
   return (int)max((int64_t)1, min((int64_t)p.shares, total / kMinShare));
 }
 
-// The item that holds unit u of all, and the unit it starts at; false past the last.
+// Share `id` of the items' units, [s, e), and the item that holds its first unit
+// with the unit that item starts at; false past the last share.
+struct Share {
+  int64_t s, e, start;
+  int item;
+};
 template <bool SEL>
-__device__ __forceinline__ bool item_at(const AttendK& p, int64_t u, int lane, int* item, int64_t* start) {
+__device__ __forceinline__ bool share_at(const AttendK& p, int id, int lane, Share* out) {
+  const uint32_t n0 = item_units<SEL>(p, lane), incl0 = wave_prefix(n0, lane);   // of the first 64 items
+  int64_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl0, kWave - 1);
+  for (int i0 = kWave; i0 < p.items; i0 += kWave) total += (uint32_t)wave_sum_int((int)item_units<SEL>(p, i0 + lane));
+  const int n = share_count(p, total);
+  if (id >= n) return false;
+  out->s = total * id / n;
+  out->e = total * (id + 1) / n;
   int64_t before = 0;
   for (int i0 = 0; i0 < p.items; i0 += kWave) {
-    const uint32_t n = item_units<SEL>(p, i0 + lane), incl = wave_prefix(n, lane);
-    const uint64_t past = __ballot(before + (int64_t)incl > u);
+    const uint32_t v = i0 == 0 ? n0 : item_units<SEL>(p, i0 + lane);
+    const uint32_t incl = i0 == 0 ? incl0 : wave_prefix(v, lane);
+    const uint64_t past = __ballot(before + (int64_t)incl > out->s);
     if (past) {
       const int i = __ffsll((long long)past) - 1;
-      *item = __builtin_amdgcn_readfirstlane(i0 + i);
-      *start = before + (uint32_t)__builtin_amdgcn_readlane((int)(incl - n), i);
+      out->item = __builtin_amdgcn_readfirstlane(i0 + i);
+      out->start = before + (uint32_t)__builtin_amdgcn_readlane((int)(incl - v), i);
       return true;
     }
     before += (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
@@ -310,8 +318,11 @@ __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile&
         for (int j = 0; j < 4; ++j) b.v[4 * e + j] = *reinterpret_cast<const VB*>(vp + (int64_t)j * a.v_st);
       }
     };
+    // (in this order, as in the loop: the wait for K then leaves V in flight)
     load_k(0);
+    __builtin_amdgcn_sched_barrier(0);
     load_v(0);
+    __builtin_amdgcn_sched_barrier(0);
     for (int i = 0; i < cnt; ++i) {
       // S^T
       f32x4_t sc[2];
@@ -327,6 +338,7 @@ __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile&
         }
       }
       load_k(i + 1);
+      __builtin_amdgcn_sched_barrier(0);
       float z[8];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -338,6 +350,7 @@ __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile&
       if (per_lane(!((whole_bits >> i) & 1))) {
         // some key is not visible to some row: its logit is -inf, and a key no
         // row sees has its V bytes cleared (0 * NaN would reach O)
+        asm volatile("");                        // (a branch: not computed and selected for every unit)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int key = __builtin_amdgcn_readlane(dk[e], i) ;
@@ -477,20 +490,27 @@ template <typename T, int KV, int D, bool SEL, int NW>
 __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3))) void cache8_decode_kernel(AttendK p) {
   const srswa_cache8_attend_args& a = p.a;
   const int lane = threadIdx.x % kWave;
-  const int h = (int)blockIdx.x % a.HKV, id = (int)blockIdx.x / a.HKV;
+  int h, id;
+  if (D == 64 && p.pairs) {
+    // two heads' rows share a 128-byte line: both on one XCD, so it is fetched once
+    const int half = a.HKV / 2, pair = (int)blockIdx.x / 16 * 8 + (int)blockIdx.x % 8;
+    h = pair % half * 2 + (int)(blockIdx.x / 8 & 1);
+    id = pair / half;
+    if (id >= (p.shares > 0 ? p.shares : p.items)) return;
+  } else {
+    h = (int)blockIdx.x % a.HKV;
+    id = (int)blockIdx.x / a.HKV;
+  }
   if (p.shares == 0) {
     const Tile t = tile_of<SEL>(p, id / p.tiles, id % p.tiles);
     if (t.nrows > 0) attend_item<T, KV, D, SEL, NW>(p, h, t, 0, t.units, nullptr);
     return;
   }
-  const int64_t total = all_units<SEL>(p, lane);
-  const int n = share_count(p, total);
-  if (id >= n) return;
-  int64_t s = total * id / n;
-  const int64_t e = total * (id + 1) / n;
-  int item;
-  int64_t start;
-  if (!item_at<SEL>(p, s, lane, &item, &start)) return;
+  Share sh;
+  if (!share_at<SEL>(p, id, lane, &sh)) return;
+  int64_t s = sh.s, start = sh.start;
+  const int64_t e = sh.e;
+  int item = sh.item;
   float* recs = p.part + ((int64_t)id * a.HKV + h) * 2 * p.rs * (D + 2);
   for (bool first = true; s < e; ++item) {
     const Tile t = tile_of<SEL>(p, item / p.tiles, item % p.tiles);
@@ -631,8 +651,11 @@ int cache8_check(const srswa_cache8_attend_args* a, const char* what) {
 
 namespace {
 
-// Items of at most 64 units (2,048 keys) are taken whole where they make 128
-// workgroups; others are shared by as many workgroups as the GPU holds at once.
+// Short items are taken whole, others shared by as many workgroups as the GPU holds
+// at once.  Whole needs no second launch and no count of the items, but leaves CUs
+// idle where the workgroups are few: one request of ten heads 9.6 us whole against
+// 15.2 shared at 777 keys, 21.5 against 16.8 at 3,000 (94 units); 24 requests of
+// 400 to 3,000 keys 23 against 31.
 AttendK plan(const srswa_cache8_attend_args* a) {
   AttendK p{};
   p.a = *a;
@@ -648,10 +671,11 @@ AttendK plan(const srswa_cache8_attend_args* a) {
   else if (a->window > 0)
     groups = std::min<int64_t>(groups, ((int64_t)a->window + a->max_query_len) / kGroup + 2 + (a->sinks + kGroup - 1) / kGroup);
   const int64_t units = (groups + 1) / 2, wgs = (int64_t)p.items * a->HKV;
+  p.pairs = a->D == 64 && a->HKV % 2 == 0;
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
-  if (units > 64 || (units > kMinShare && wgs < 128))
-    p.shares = (int)std::min<int64_t>(std::max(1, 3 * cus / a->HKV), (units * p.items + kMinShare - 1) / kMinShare);
+  if (units > 128 || (units > 64 && wgs < 40))
+    p.shares = (int)std::min<int64_t>(std::max(1, (a->D == 64 ? 4 : 3) * cus / a->HKV), (units * p.items + kMinShare - 1) / kMinShare);
   return p;
 }
 
@@ -691,7 +715,8 @@ int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_byt
     return SRSWA_WORKSPACE;
   }
   p.part = reinterpret_cast<float*>(ws);
-  const int64_t grid = (int64_t)(p.shares > 0 ? p.shares : p.items) * a->HKV;
+  const int64_t wgs = (int64_t)(p.shares > 0 ? p.shares : p.items) * a->HKV;
+  const int64_t grid = p.pairs ? (wgs / 2 + 7) / 8 * 16 : wgs;
   if (grid > 0x7fffffff || (int64_t)a->R * p.tiles * a->HKV * p.rs > 0x7fffffff) {
     set_error("%s: grid too large", what);
     return SRSWA_UNSUPPORTED;
