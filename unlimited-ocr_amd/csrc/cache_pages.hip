@@ -43,8 +43,7 @@ __device__ __forceinline__ int block_sum(int v, int* s) {
   if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = v;
   __syncthreads();
   int t = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / kWave; ++w) t += s[w];
+  for (int w = 0; w < (int)blockDim.x / kWave; ++w) t += s[w];
   return t;
 }
 
@@ -61,8 +60,7 @@ __device__ __forceinline__ int block_scan(int v, int* s, int* total) {
   if (lane == kWave - 1) s[w] = incl;
   __syncthreads();
   int base = 0, t = 0;
-#pragma unroll
-  for (int i = 0; i < kThreads / kWave; ++i) {
+  for (int i = 0; i < (int)blockDim.x / kWave; ++i) {
     base += i < w ? s[i] : 0;
     t += s[i];
   }
@@ -75,7 +73,7 @@ __device__ __forceinline__ bool valid_page(const PagesK& p, int id) { return id 
 // Marks and counts the free pages of one tile of ref.
 __device__ __forceinline__ void mark_tile(const PagesK& p, const int32_t* ref, int tile, int* s) {
   int n = 0;
-  for (int i = threadIdx.x; i < kTile; i += kThreads) {
+  for (int i = threadIdx.x; i < kTile; i += (int)blockDim.x) {
     const int page = tile * kTile + i;
     const bool fr = page < p.N && ref[page] == 0;
     const uint64_t b = __ballot(fr);
@@ -86,35 +84,45 @@ __device__ __forceinline__ void mark_tile(const PagesK& p, const int32_t* ref, i
   if (threadIdx.x == 0) p.tfree[tile] = n;
 }
 
-// The free pages of ranks [k0, k0 + n): put(k, page) for each that exists, from
-// the tile counts and the bitmap.  Every thread of the workgroup calls it.
+// The free pages of ranks [k0, k0 + n): put(k, page) for each that exists.  The
+// tiles that hold them are found from the tile counts; a wave then takes a tile, a
+// lane each of its 64 words.  Every thread of the workgroup calls it.
+struct Hit {
+  int tile, before;
+};
 template <typename Put>
-__device__ __forceinline__ void find_free(const PagesK& p, int k0, int n, int* s, Put put) {
+__device__ __forceinline__ void find_free(const PagesK& p, int k0, int n, int* s, Hit* s_hit, int* s_nhit, Put put) {
+  static_assert(kTile == 32 * kWave, "a lane per word of a tile");
   int before = 0;
-  for (int t0 = 0; t0 < p.ntiles && before < k0 + n; t0 += kThreads) {
+  for (int t0 = 0; t0 < p.ntiles && before < k0 + n; t0 += (int)blockDim.x) {
+    if (threadIdx.x == 0) *s_nhit = 0;
     const int t = t0 + threadIdx.x;
     const int c = t < p.ntiles ? p.tfree[t] : 0;
     int total;
     const int b = before + block_scan(c, s, &total);
-    // one thread per tile walks its words; the tiles that hold a wanted rank are few
-    if (c > 0 && b < k0 + n && b + c > k0) {
-      int k = b;
-      const int w1 = min((t + 1) * (kTile / 32), (p.N + 31) / 32);
-      for (int w = t * (kTile / 32); w < w1 && k < k0 + n; ++w) {
-        uint32_t x = p.bits[w];
-        const int m = __popc(x);
-        if (k + m <= k0) {
-          k += m;
-          continue;
-        }
+    if (c > 0 && b < k0 + n && b + c > k0) s_hit[atomicAdd(s_nhit, 1)] = Hit{t, b};   // (any order)
+    __syncthreads();
+    const int hits = *s_nhit, lane = threadIdx.x % kWave;
+    for (int i = threadIdx.x / kWave; i < hits; i += (int)blockDim.x / kWave) {
+      const int w = s_hit[i].tile * kWave + lane;
+      uint32_t x = w < (p.N + 31) / 32 ? p.bits[w] : 0u;
+      const int m = __popc(x);
+      int incl = m;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int v = __shfl_up(incl, o, kWave);
+        if (lane >= o) incl += v;
+      }
+      int k = s_hit[i].before + incl - m;
+      if (k + m > k0 && k < k0 + n)
         while (x) {
           const int bit = __ffs((int)x) - 1;
           x &= x - 1;
           if (k >= k0 && k < k0 + n) put(k, w * 32 + bit);
           ++k;
         }
-      }
     }
+    __syncthreads();
     before += total;
   }
 }
@@ -169,6 +177,8 @@ __global__ __launch_bounds__(kThreads) void reserve_deal_kernel(PagesK p) {
     if (need == 0) return;
   }
   // the row's missing entries in order: entry of rank k takes the free page of rank before + k
+  __shared__ Hit s_hit[kThreads];
+  __shared__ int s_nhit;
   const int nb = (int)min((int64_t)p.W, ((int64_t)max(p.rows[r], 0) + p.page_size - 1) / p.page_size);
   __shared__ int s_blk[kThreads];
   int done = 0;
@@ -180,7 +190,7 @@ __global__ __launch_bounds__(kThreads) void reserve_deal_kernel(PagesK p) {
     if (miss) s_blk[k] = b;
     __syncthreads();
     if (got > 0)
-      find_free(p, before + done, got, s, [&](int rank, int page) {
+      find_free(p, before + done, got, s, s_hit, &s_nhit, [&](int rank, int page) {
         p.bto[(int64_t)r * p.bto_sr + s_blk[rank - before - done]] = page;
         p.refo[page] = 1;
       });
@@ -195,53 +205,48 @@ __global__ __launch_bounds__(kThreads) void copy_ref_kernel(PagesK p) {
   if (i < p.N) p.refo[i] = p.ref[i];
 }
 
-// rows: the parents.  A workgroup per row writes its new entries, moves the
-// references from its old pages to its new ones and notes the page it must copy.
-__global__ __launch_bounds__(kThreads) void reorder_rows_kernel(PagesK p) {
-  __shared__ int s[kThreads / kWave];
-  const int r = (int)blockIdx.x;
-  const int par = p.rows[r];
+// rows: the parents.  `threads` threads write row r's new entries, move the
+// references from its old pages to its new ones; returns the page it must copy (-1:
+// none) to the first of them.
+__device__ __forceinline__ int reorder_row(const PagesK& p, int r, int par, int len, int me, int threads, bool first) {
   const bool alive = par >= 0 && par < p.R;
-  int older = 0;
-  for (int i = threadIdx.x; alive && i < r; i += kThreads) older += p.rows[i] == par;
-  older = block_sum(older, s);
-  const bool first = alive && older == 0;
-  const int len = alive ? p.sl[par] : 0;
   const int full = max(len, 0) / p.page_size;
   const int begun = max(len, 0) % p.page_size;
-  for (int b = threadIdx.x; b < p.W; b += kThreads) {
-    const int old = p.bt[(int64_t)r * p.bt_sr + b];
-    const int id = alive ? p.bt[(int64_t)par * p.bt_sr + b] : -1;
-    const bool keep = alive && (first || b < full);
-    const int now = keep ? id : -1;
-    p.bto[(int64_t)r * p.bto_sr + b] = now;
-    if (old != now) {
-      if (valid_page(p, old)) atomicSub(&p.refo[old], 1);
-      if (valid_page(p, now)) atomicAdd(&p.refo[now], 1);
+  const int32_t* mine = p.bt + (int64_t)r * p.bt_sr;
+  const int32_t* theirs = p.bt + (int64_t)(alive ? par : r) * p.bt_sr;
+  int src = -1;                                   // (its load is in flight beside the first entries')
+  if (me == 0 && alive && !first && begun > 0 && full < p.W) src = theirs[full];
+  for (int b0 = me; b0 < p.W; b0 += 8 * threads) {
+    int old[8], id[8];                            // (loaded together, before any addition)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int b = min(b0 + k * threads, p.W - 1);
+      old[k] = mine[b];
+      id[k] = theirs[b];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int b = b0 + k * threads;
+      if (b >= p.W) break;
+      const int now = alive && (first || b < full) ? id[k] : -1;
+      p.bto[(int64_t)r * p.bto_sr + b] = now;
+      if (old[k] != now) {
+        if (valid_page(p, old[k])) atomicSub(&p.refo[old[k]], 1);
+        if (valid_page(p, now)) atomicAdd(&p.refo[now], 1);
+      }
     }
   }
-  if (threadIdx.x == 0) {
-    p.slo[r] = len;
-    int src = -1;
-    if (alive && !first && begun > 0 && full < p.W) src = p.bt[(int64_t)par * p.bt_sr + full];
-    p.src[r] = valid_page(p, src) ? src : -1;
-  }
+  if (me == 0) p.slo[r] = len;
+  return valid_page(p, src) ? src : -1;
 }
 
-__global__ __launch_bounds__(kThreads) void mark_kernel(PagesK p) {
-  __shared__ int s[kThreads / kWave];
-  mark_tile(p, p.refo, (int)blockIdx.x, s);
-}
-
-// One workgroup deals free pages to the rows that copy, in row order.
-__global__ __launch_bounds__(kThreads) void reorder_deal_kernel(PagesK p) {
-  __shared__ int s[kThreads / kWave];
-  __shared__ int s_row[kThreads];
+// Deals free pages to the rows that copy, in row order (one workgroup).
+__device__ __forceinline__ void reorder_deal(const PagesK& p, int* s, int* s_row, Hit* s_hit, int* s_nhit) {
   int fr = 0;
-  for (int i = threadIdx.x; i < p.ntiles; i += kThreads) fr += p.tfree[i];
+  for (int i = threadIdx.x; i < p.ntiles; i += (int)blockDim.x) fr += p.tfree[i];
   fr = block_sum(fr, s);
   int done = 0;
-  for (int r0 = 0; r0 < p.R; r0 += kThreads) {
+  for (int r0 = 0; r0 < p.R; r0 += (int)blockDim.x) {
     const int r = r0 + threadIdx.x;
     const bool want = r < p.R && p.src[r] >= 0;
     int n;
@@ -250,7 +255,7 @@ __global__ __launch_bounds__(kThreads) void reorder_deal_kernel(PagesK p) {
     if (r < p.R) p.dst[r] = -1;
     __syncthreads();
     if (n > 0)
-      find_free(p, done, n, s, [&](int rank, int page) {
+      find_free(p, done, n, s, s_hit, s_nhit, [&](int rank, int page) {
         const int row = s_row[rank - done];
         p.dst[row] = page;
         p.bto[(int64_t)row * p.bto_sr + p.slo[row] / p.page_size] = page;
@@ -261,6 +266,97 @@ __global__ __launch_bounds__(kThreads) void reorder_deal_kernel(PagesK p) {
   }
   if (threadIdx.x == 0) {
     *p.count = max(done - fr, 0);
+    *p.npairs = p.R;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void reorder_rows_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  const int r = (int)blockIdx.x, par = p.rows[r];
+  const bool alive = par >= 0 && par < p.R;
+  int older = 0;                                  // rows before this one that continue the same parent
+  for (int i = threadIdx.x; alive && i < r; i += kThreads) older += p.rows[i] == par;
+  older = block_sum(older, s);
+  const int src = reorder_row(p, r, par, alive ? p.sl[par] : 0, threadIdx.x, kThreads, older == 0);
+  if (threadIdx.x == 0) p.src[r] = src;
+}
+
+__global__ __launch_bounds__(kThreads) void mark_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  mark_tile(p, p.refo, (int)blockIdx.x, s);
+}
+
+__global__ __launch_bounds__(kThreads) void reorder_deal_kernel(PagesK p) {
+  __shared__ int s[kThreads / kWave];
+  __shared__ int s_row[kThreads];
+  __shared__ Hit s_hit[kThreads];
+  __shared__ int s_nhit;
+  reorder_deal(p, s, s_row, s_hit, &s_nhit);
+}
+
+// The four steps in one workgroup, for up to kWide rows and 32 kWide pages, the
+// marks and the list of free pages in LDS: a power of two of threads per row, every
+// row at once where they suffice (64 rows of 128 pages 13 us; the same steps through
+// memory 24 us).
+constexpr int kWide = 1024;
+__global__ __launch_bounds__(kWide) void reorder_plan_kernel(PagesK p) {
+  __shared__ int s[kWide / kWave];
+  __shared__ int s_par[kWide], s_len[kWide], s_src[kWide], s_free[kWide];
+  __shared__ uint32_t s_bits[kWide];
+  const int tid = threadIdx.x;
+  s_bits[tid] = 0u;
+  if (tid < p.R) {
+    const int par = p.rows[tid];
+    s_par[tid] = par;
+    s_len[tid] = par >= 0 && par < p.R ? p.sl[par] : 0;
+  }
+  for (int i = tid; i < p.N; i += kWide) p.refo[i] = p.ref[i];
+  __syncthreads();
+  int per = kWave;                                // threads per row
+  while (per > 1 && per * p.R > kWide) per >>= 1;
+  const int me = tid & (per - 1);
+  for (int r = tid / per; r < p.R; r += kWide / per) {
+    const int par = s_par[r];
+    int older = 0;
+    for (int i = me; i < r; i += per) older += s_par[i] == par;
+    for (int o = 1; o < per; o <<= 1) older += __shfl_xor(older, o, kWave);
+    const int src = reorder_row(p, r, par, s_len[r], me, per, older == 0);
+    if (me == 0) {
+      s_src[r] = src;
+      p.src[r] = src;
+    }
+  }
+  __syncthreads();                                // (orders this workgroup's global accesses too)
+  for (int i0 = 0; i0 < p.N; i0 += kWide) {
+    // the additions went past this CU's cache: so does the load
+    const int i = i0 + tid;
+    const bool fr = i < p.N && __hip_atomic_load(p.refo + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0;
+    const uint64_t b = __ballot(fr);
+    if (tid % 32 == 0) s_bits[i / 32] = (uint32_t)(tid % kWave ? b >> 32 : b);
+  }
+  __syncthreads();
+  // the rank of a row that copies among them, and the free page of that rank
+  int wants, nfree;
+  const bool want = tid < p.R && s_src[tid] >= 0;
+  const int rank = block_scan(want ? 1 : 0, s, &wants);
+  uint32_t x = s_bits[tid];
+  int k = block_scan(__popc(x), s, &nfree);
+  while (x && k < wants) {
+    const int bit = __ffs((int)x) - 1;
+    x &= x - 1;
+    s_free[k++] = tid * 32 + bit;
+  }
+  __syncthreads();
+  if (tid < p.R) {
+    const int page = want && rank < nfree ? s_free[rank] : -1;
+    p.dst[tid] = page;
+    if (page >= 0) {
+      p.bto[(int64_t)tid * p.bto_sr + s_len[tid] / p.page_size] = page;
+      p.refo[page] = 1;
+    }
+  }
+  if (tid == 0) {
+    *p.count = max(wants - nfree, 0);
     *p.npairs = p.R;
   }
 }
@@ -346,34 +442,58 @@ __global__ __launch_bounds__(kThreads) void compact_table_kernel(PagesK p, int r
 // ---------------------------------------------------------------- copy
 struct CopyK {
   srswa_page_cache c[kMaxCaches];
-  int n;                        // caches
+  int n, big;                   // caches; the first `big` are cut into slices of kSlice bytes
+  int slices;                   // of the largest
   const int32_t* src;
   const int32_t* dst;
   const int32_t* npairs;
   int N;
 };
 
-// Workgroups take (pair, cache) items in turn; a pair whose destination is -1
-// copies nothing.  No destination is a source (a source is held, a destination
-// was free), so the order does not matter.
+constexpr int kSlice = kThreads * 4 * 16;
+
+// Workgroups take (pair, cache, slice) items of the big caches in turn, four
+// 16-byte loads a thread in flight, then pairs whose small caches a wave each
+// copies.  A pair whose destination is -1 copies nothing.  No destination is a
+// source (a source is held, a destination was free), so the order does not matter.
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyK p) {
-  const int64_t items = (int64_t)*p.npairs * p.n;
+  const int np = *p.npairs;
+  auto pair = [&](int i, int* s, int* d) {
+    *s = p.src[i];
+    *d = p.dst[i];
+    return *s >= 0 && *s < p.N && *d >= 0 && *d < p.N;
+  };
+  const int64_t items = (int64_t)np * p.big * p.slices;
+  int s, d;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int i = (int)(it / p.n);
-    const int s = p.src[i], d = p.dst[i];
-    if (s < 0 || s >= p.N || d < 0 || d >= p.N) continue;
-    const srswa_page_cache c = p.c[it % p.n];
-    const unsigned char* from = reinterpret_cast<const unsigned char*>(c.base) + (int64_t)s * c.stride;
-    unsigned char* to = reinterpret_cast<unsigned char*>(c.base) + (int64_t)d * c.stride;
-    const uint64_t al = reinterpret_cast<uintptr_t>(c.base) | (uint64_t)c.stride | (uint64_t)c.bytes;
-    if (al % 16 == 0) {
-      for (int64_t k = threadIdx.x; k < c.bytes / 16; k += kThreads)
-        reinterpret_cast<uint4*>(to)[k] = reinterpret_cast<const uint4*>(from)[k];
-    } else if (al % 4 == 0) {
-      for (int64_t k = threadIdx.x; k < c.bytes / 4; k += kThreads)
+    const int sl = (int)(it % p.slices);
+    const int64_t ic = it / p.slices;
+    const srswa_page_cache c = p.c[ic % p.big];
+    if (!pair((int)(ic / p.big), &s, &d) || (int64_t)sl * kSlice >= c.bytes) continue;
+    const int n = (int)min((int64_t)kSlice, c.bytes - (int64_t)sl * kSlice) / 16;
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const char*>(c.base) + (int64_t)s * c.stride + (int64_t)sl * kSlice);
+    uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(c.base) + (int64_t)d * c.stride + (int64_t)sl * kSlice);
+    const int i = threadIdx.x, last = n - 1;
+    const uint4 v0 = from[min(i, last)], v1 = from[min(i + kThreads, last)], v2 = from[min(i + 2 * kThreads, last)],
+                v3 = from[min(i + 3 * kThreads, last)];
+    if (i < n) to[i] = v0;
+    if (i + kThreads < n) to[i + kThreads] = v1;
+    if (i + 2 * kThreads < n) to[i + 2 * kThreads] = v2;
+    if (i + 3 * kThreads < n) to[i + 3 * kThreads] = v3;
+  }
+  const int small = p.n - p.big, lane = threadIdx.x % kWave;
+  const int64_t parts = (int64_t)np * small;
+  for (int64_t it = (int64_t)blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave; it < parts;
+       it += (int64_t)gridDim.x * (kThreads / kWave)) {
+    const srswa_page_cache c = p.c[p.big + it % small];
+    if (!pair((int)(it / small), &s, &d)) continue;
+    const char* from = static_cast<const char*>(c.base) + (int64_t)s * c.stride;
+    char* to = static_cast<char*>(c.base) + (int64_t)d * c.stride;
+    if (((reinterpret_cast<uintptr_t>(c.base) | (uint64_t)c.stride | (uint64_t)c.bytes) & 3) == 0) {
+      for (int64_t k = lane; k < c.bytes / 4; k += kWave)
         reinterpret_cast<uint32_t*>(to)[k] = reinterpret_cast<const uint32_t*>(from)[k];
     } else {
-      for (int64_t k = threadIdx.x; k < c.bytes; k += kThreads) to[k] = from[k];
+      for (int64_t k = lane; k < c.bytes; k += kWave) to[k] = from[k];
     }
   }
 }
@@ -437,14 +557,29 @@ int setup(const srswa_pages_args* a, void* ws, size_t ws_bytes, bool rows, const
   return SRSWA_OK;
 }
 
+// A cache whose pages are 16-byte aligned and hold 2 KB or more is cut into slices,
+// any other copied by a wave a page.
+bool is_big(const srswa_page_cache& c) {
+  return ((reinterpret_cast<uintptr_t>(c.base) | (uint64_t)c.stride | (uint64_t)c.bytes) & 15) == 0 && c.bytes >= 2048;
+}
+
 void copy_pages(const srswa_pages_args* a, const PagesK& k, int64_t most_pairs, hipStream_t st) {
   for (int c0 = 0; c0 < a->ncaches; c0 += kMaxCaches) {
     CopyK c{};
-    c.n = std::min(kMaxCaches, a->ncaches - c0);
-    for (int i = 0; i < c.n; ++i) c.c[i] = a->caches[c0 + i];
+    c.slices = 1;
+    const int n = std::min(kMaxCaches, a->ncaches - c0);
+    for (int big = 1; big >= 0; --big)
+      for (int i = 0; i < n; ++i)
+        if (is_big(a->caches[c0 + i]) == (big == 1)) {
+          c.c[c.n++] = a->caches[c0 + i];
+          if (big) {
+            c.big = c.n;
+            c.slices = std::max(c.slices, (int)((a->caches[c0 + i].bytes + kSlice - 1) / kSlice));
+          }
+        }
     c.src = k.src;  c.dst = k.dst;  c.npairs = k.npairs;  c.N = k.N;
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most_pairs * c.n, 2048));
-    copy_pages_kernel<<<grid, kThreads, 0, st>>>(c);
+    const int64_t items = most_pairs * std::max<int64_t>((int64_t)c.big * c.slices, (c.n - c.big + 3) / 4);
+    copy_pages_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(items, 8192)), kThreads, 0, st>>>(c);
   }
 }
 
@@ -481,10 +616,14 @@ extern "C" int srswa_pages_reorder(const srswa_pages_args* a, void* ws, size_t w
   const int rc = setup(a, ws, ws_bytes, true, "pages reorder", &k);
   if (rc != SRSWA_OK) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  copy_ref_kernel<<<(unsigned)((k.N + kThreads - 1) / kThreads), kThreads, 0, st>>>(k);
-  reorder_rows_kernel<<<(unsigned)k.R, kThreads, 0, st>>>(k);
-  mark_kernel<<<(unsigned)k.ntiles, kThreads, 0, st>>>(k);
-  reorder_deal_kernel<<<1, kThreads, 0, st>>>(k);
+  if (k.R <= kWide && (int64_t)k.R * k.W <= 32768 && k.N <= 32 * kWide) {
+    reorder_plan_kernel<<<1, kWide, 0, st>>>(k);
+  } else {
+    copy_ref_kernel<<<(unsigned)((k.N + kThreads - 1) / kThreads), kThreads, 0, st>>>(k);
+    reorder_rows_kernel<<<(unsigned)k.R, kThreads, 0, st>>>(k);
+    mark_kernel<<<(unsigned)k.ntiles, kThreads, 0, st>>>(k);
+    reorder_deal_kernel<<<1, kThreads, 0, st>>>(k);
+  }
   copy_pages(a, k, k.R, st);
   return done("pages reorder");
 }
