@@ -85,19 +85,21 @@ __device__ __forceinline__ void mark_tile(const PagesK& p, const int32_t* ref, i
 }
 
 // The free pages of ranks [k0, k0 + n): put(k, page) for each that exists.  The
-// tiles that hold them are found from the tile counts; a wave then takes a tile, a
+// tiles that hold them are found from the tile counts (c0: tile threadIdx.x's); a
+// wave then takes a tile, a
 // lane each of its 64 words.  Every thread of the workgroup calls it.
 struct Hit {
   int tile, before;
 };
 template <typename Put>
-__device__ __forceinline__ void find_free(const PagesK& p, int k0, int n, int* s, Hit* s_hit, int* s_nhit, Put put) {
+__device__ __forceinline__ void find_free(const PagesK& p, int k0, int n, int c0, int* s, Hit* s_hit, int* s_nhit,
+                                          Put put) {
   static_assert(kTile == 32 * kWave, "a lane per word of a tile");
   int before = 0;
   for (int t0 = 0; t0 < p.ntiles && before < k0 + n; t0 += (int)blockDim.x) {
     if (threadIdx.x == 0) *s_nhit = 0;
     const int t = t0 + threadIdx.x;
-    const int c = t < p.ntiles ? p.tfree[t] : 0;
+    const int c = t0 == 0 ? c0 : t < p.ntiles ? p.tfree[t] : 0;
     int total;
     const int b = before + block_scan(c, s, &total);
     if (c > 0 && b < k0 + n && b + c > k0) s_hit[atomicAdd(s_nhit, 1)] = Hit{t, b};   // (any order)
@@ -155,15 +157,23 @@ __global__ __launch_bounds__(kThreads) void reserve_count_kernel(PagesK p) {
   }
 }
 
-// Second launch: each row that misses pages takes the free pages of its ranks.
+// Second launch: each row that misses pages takes the free pages of its ranks.  What
+// the first thread-width of rows, tiles and entries needs is loaded at once, before
+// any of it is used.
 __global__ __launch_bounds__(kThreads) void reserve_deal_kernel(PagesK p) {
   __shared__ int s[kThreads / kWave];
-  const int r = (int)blockIdx.x;
-  int before = 0, all = 0, fr = 0;
+  __shared__ int s_blk[kThreads];
+  __shared__ Hit s_hit[kThreads];
+  __shared__ int s_nhit;
+  const int r = (int)blockIdx.x, tid = threadIdx.x;
   const bool last = r == p.R - 1;
-  const int need = p.need[r];
+  const int need = p.need[r], len = p.rows[r];
+  const int n0 = tid < p.R ? p.need[tid] : 0;
+  const int c0 = tid < p.ntiles ? p.tfree[tid] : 0;
+  const int e0 = p.bt[(int64_t)r * p.bt_sr + min(tid, p.W - 1)];
   if (need == 0 && !last) return;
-  for (int i = threadIdx.x; i < p.R; i += kThreads) {
+  int before = tid < r ? n0 : 0, all = n0, fr = c0;
+  for (int i = tid + kThreads; i < p.R; i += kThreads) {
     const int n = p.need[i];
     before += i < r ? n : 0;
     all += n;
@@ -171,26 +181,23 @@ __global__ __launch_bounds__(kThreads) void reserve_deal_kernel(PagesK p) {
   before = block_sum(before, s);
   if (last) {
     all = block_sum(all, s);
-    for (int i = threadIdx.x; i < p.ntiles; i += kThreads) fr += p.tfree[i];
+    for (int i = tid + kThreads; i < p.ntiles; i += kThreads) fr += p.tfree[i];
     fr = block_sum(fr, s);
-    if (threadIdx.x == 0) *p.count = max(all - fr, 0);
+    if (tid == 0) *p.count = max(all - fr, 0);
     if (need == 0) return;
   }
   // the row's missing entries in order: entry of rank k takes the free page of rank before + k
-  __shared__ Hit s_hit[kThreads];
-  __shared__ int s_nhit;
-  const int nb = (int)min((int64_t)p.W, ((int64_t)max(p.rows[r], 0) + p.page_size - 1) / p.page_size);
-  __shared__ int s_blk[kThreads];
+  const int nb = (int)min((int64_t)p.W, ((int64_t)max(len, 0) + p.page_size - 1) / p.page_size);
   int done = 0;
   for (int b0 = 0; b0 < nb && done < need; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    const bool miss = b < nb && p.bt[(int64_t)r * p.bt_sr + b] < 0;
+    const int b = b0 + tid;
+    const bool miss = b < nb && (b0 == 0 ? e0 : p.bt[(int64_t)r * p.bt_sr + b]) < 0;
     int got;
     const int k = block_scan(miss ? 1 : 0, s, &got);
     if (miss) s_blk[k] = b;
     __syncthreads();
     if (got > 0)
-      find_free(p, before + done, got, s, s_hit, &s_nhit, [&](int rank, int page) {
+      find_free(p, before + done, got, c0, s, s_hit, &s_nhit, [&](int rank, int page) {
         p.bto[(int64_t)r * p.bto_sr + s_blk[rank - before - done]] = page;
         p.refo[page] = 1;
       });
@@ -255,7 +262,7 @@ __device__ __forceinline__ void reorder_deal(const PagesK& p, int* s, int* s_row
     if (r < p.R) p.dst[r] = -1;
     __syncthreads();
     if (n > 0)
-      find_free(p, done, n, s, s_hit, s_nhit, [&](int rank, int page) {
+      find_free(p, done, n, (int)threadIdx.x < p.ntiles ? p.tfree[threadIdx.x] : 0, s, s_hit, s_nhit, [&](int rank, int page) {
         const int row = s_row[rank - done];
         p.dst[row] = page;
         p.bto[(int64_t)row * p.bto_sr + p.slo[row] / p.page_size] = page;
