@@ -285,10 +285,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   settle(qf);
   __syncthreads();
   // one chunk: the next one (in f) goes to the other buffer, f takes the third next
+  // (converted last, beside the last products: first, the window case took 5% longer)
   auto step = [&](int u, int buf, Fetched& f) __attribute__((always_inline)) {
-    stage(min(u + 1, u_hi - 1), buf ^ 1, f);
-    fetch(u + 3, f);
-    pgn = page_of(u + 4);
     const uint16_t* sK = reinterpret_cast<const uint16_t*>(smem + buf * L::buf);
     const uint16_t* sV = reinterpret_cast<const uint16_t*>(smem + buf * L::buf + L::kBytes);
     const float4* sg = reinterpret_cast<const float4*>(smem + buf * L::buf + L::kBytes + L::vBytes);
@@ -364,6 +362,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             o[d] = Mfma<__half>::mac(a_operand_tr<VP>(sV, 32 * kt + 16 * q, 32 * d, lane), pf, o[d]);
         }
     }
+    stage(min(u + 1, u_hi - 1), buf ^ 1, f);
+    fetch(u + 3, f);
+    pgn = page_of(u + 4);
     __syncthreads();
   };
   for (int u = u_lo; u < u_hi; u += 2) {
