@@ -49,6 +49,7 @@ struct AttendK {
   bool pairs;             // D = 64: neighbouring heads to one XCD
   int rs;                 // rows of a record
   int gpp;                // 16-key groups per page
+  int64_t most_units;     // of an item
   float scale_l2;         // scale * log2(e)
   float* part;            // records: [shares][HKV][2][rs * (D + 2)], a share's first item and its last
 };
@@ -671,6 +672,7 @@ AttendK plan(const srswa_cache8_attend_args* a) {
   else if (a->window > 0)
     groups = std::min<int64_t>(groups, ((int64_t)a->window + a->max_query_len) / kGroup + 2 + (a->sinks + kGroup - 1) / kGroup);
   const int64_t units = (groups + 1) / 2, wgs = (int64_t)p.items * a->HKV;
+  p.most_units = units;
   p.pairs = a->D == 64 && a->HKV % 2 == 0;
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
@@ -728,6 +730,12 @@ int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_byt
 }
 
 size_t cache8_decode_ws(const srswa_cache8_attend_args* a) { return ws_bytes_of(plan(a)); }
+
+void cache8_decode_load(const srswa_cache8_attend_args* a, int64_t* wgs, int64_t* units) {
+  const AttendK p = plan(a);
+  *wgs = (int64_t)p.items * a->HKV;
+  *units = p.most_units;
+}
 
 }  // namespace srswa
 

@@ -28,6 +28,7 @@ constexpr int kThreads = 256;
 constexpr int kRowsWg = 128;
 constexpr int kGroup = 16;
 constexpr int kXcds = 8;
+constexpr int kMinChunks = 4;
 constexpr float kBelow = 7.f, kSlack = 8.f;
 
 struct PrefillK {
@@ -113,9 +114,9 @@ __device__ __forceinline__ bool nth_tile(const PrefillK& p, int b, int lane, int
   return false;
 }
 
-// Parts of a tile: at least eight chunks each.
+// Parts of a tile: at least kMinChunks chunks each.
 __device__ __forceinline__ int parts_of(const PrefillK& p, const Tile& t) {
-  return max(1, min(p.nsplit, t.chunks / 8));
+  return max(1, min(p.nsplit, t.chunks / kMinChunks));
 }
 
 template <typename T, int KV, int D, bool ONE>
@@ -447,8 +448,9 @@ __global__ __launch_bounds__(2 * D) void cache8_join_kernel(PrefillK p) {
 }
 
 // Parts: the fewest that need the least rounds of the GPU per part, where two
-// workgroups share a CU and a (request, head, part)'s tiles an XCD; eight chunks
-// of a full table are one part's least.
+// workgroups share a CU and a (request, head, part)'s tiles an XCD; four chunks of a
+// full table are one part's least (eight requests of 128 rows after up to 2,000 keys
+// 47 us with eight, 35 with four, 36 with two; of 512 rows alone 31, 31, 53).
 PrefillK plan(const srswa_cache8_attend_args* a) {
   PrefillK p{};
   p.a = *a;
@@ -461,7 +463,7 @@ PrefillK plan(const srswa_cache8_attend_args* a) {
   p.page_mul = (uint32_t)(((1ull << (31 + lg)) / a->page_size) + 1);
   int64_t keys = (int64_t)a->max_blocks * a->page_size;
   if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + kRowsWg / p.G + 2 * kChunk + a->sinks);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, keys / kChunk / 8));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, keys / kChunk / kMinChunks));
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
   // rounds of the GPU per part, tiles dealt in turn (half a tile per request is a
@@ -489,8 +491,20 @@ size_t ws_bytes_of(const PrefillK& p) {
   return p.nsplit > 1 ? (size_t)p.groups * p.tiles * kRowsWg * (p.a.D + 2) * sizeof(float) : 0;
 }
 
-// Few rows per request take the form split over the keys.
-bool narrow(const srswa_cache8_attend_args* a) { return (int64_t)a->max_query_len * (a->HQ / a->HKV) <= 32; }
+// Few rows per request, or little work in all, take decode's form of 16-row items: a
+// 128-row tile converts each key once for eight times the rows, but fills fewer CUs
+// and takes longer to start and to end.  One request of ten heads, 16-row items against tiles: 49 against
+// 68 us (32 rows after 30,720 keys), 104 against 75 (128 rows), 11.5 against 22
+// (512 rows, no prefix); eight requests: 24.6 against 35 (64 rows after up to 2,000
+// keys), 41 against 31 (512 rows, no prefix).
+bool narrow(const srswa_cache8_attend_args* a) {
+  if ((int64_t)a->max_query_len * (a->HQ / a->HKV) <= 32) return true;
+  int64_t wgs, units;
+  cache8_decode_load(a, &wgs, &units);
+  int cus = device_cu_count();
+  if (cus <= 0) cus = 256;
+  return wgs <= 3 * cus && wgs * units <= 156 * cus;
+}
 
 template <typename T, int KV, int D, bool ONE>
 int launch_tiles(const PrefillK& p, unsigned grid, hipStream_t st) {
