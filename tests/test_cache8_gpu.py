@@ -433,6 +433,177 @@ def test_empty_calls(dev):
     assert not kc.any() and (s == 1).all()
 
 
+# A bound above the longest request: the work it allows for takes 128-row tiles, which
+# short prompts of a tight bound do not.
+WIDE = 1 << 15
+
+
+def _prefill(dev, c, g, bound, spoil=None, q=None):
+    """(out, lse, oracle) of PREFILL-like case c; `spoil` may plant bytes in K and V."""
+    from srswa import cache8
+    lens = [a + b for a, b in zip(c["q"], c["ctx"])]
+    table, kc, vc, ks, vs = _state(c, g, lens)
+    if spoil:
+        spoil(table, kc, vc, ks, vs)
+    cu = torch.tensor([0] + c["q"]).cumsum(0).tolist()
+    q = torch.randn(cu[-1], c["HQ"], c["D"], generator=g).to(BF) if q is None else q
+    win, sinks, scale = c.get("window"), c.get("sinks", 0), c["D"] ** -0.5
+    ref = O.attend(q, kc, vc, ks, vs, table, cu, lens, scale, window=win, sinks=sinks)
+    got, lse = cache8.cache8_prefill(*(t.to(dev) for t in (q, kc, vc, ks, vs)),
+                                     torch.tensor(table, dtype=torch.int32).to(dev), torch.tensor(cu).to(dev),
+                                     torch.tensor(lens).to(dev), bound or max(c["q"]), scale=scale, window=win,
+                                     sinks=sinks, return_lse=True)
+    return got, lse, ref
+
+
+@pytest.mark.parametrize("kv", [torch.int8, E4M3])
+@pytest.mark.parametrize("name", list(PREFILL))
+def test_prefill_tiles_match_oracle(dev, name, kv):
+    g = torch.Generator().manual_seed(list(PREFILL).index(name) + 160)
+    got, lse, ref = _prefill(dev, dict(PREFILL[name], kv=kv), g, WIDE)
+    _check(got, lse, ref, name)
+
+
+@pytest.mark.parametrize("bound", [0, WIDE])
+def test_prefill_of_many_requests(dev, bound):
+    """More requests than a wave has lanes: each workgroup finds its own."""
+    g = torch.Generator().manual_seed(171)
+    n = torch.randint(0, 9, (150,), generator=g).tolist()
+    n[70], n[149] = 140, 33
+    c = dict(page=16, HQ=4, HKV=2, D=64, kv=E4M3, q=n, ctx=torch.randint(0, 20, (150,), generator=g).tolist(), W=10)
+    got, lse, ref = _prefill(dev, c, g, bound)
+    _check(got, lse, ref, "150 requests")
+
+
+def _check_nan(got, lse, ref, what):
+    o, l, tol = ref
+    got, lse = got.cpu().double(), lse.cpu().double()
+    bad, lbad = torch.isnan(o), torch.isnan(l)
+    assert bad.any(), what
+    assert torch.equal(torch.isnan(got), bad), (what, (torch.isnan(got) != bad).nonzero()[:8].tolist())
+    assert torch.equal(torch.isnan(lse), lbad), what
+    assert ((got - o).abs() <= tol)[~bad].all(), what
+    fine = ~lbad & ~torch.isinf(l)
+    assert torch.equal(torch.isinf(lse), torch.isinf(l)), what
+    assert ((lse - l).abs()[fine] <= 1e-4 * (1 + l[fine].abs())).all(), what
+
+
+NANS = {
+    "causal": dict(page=16, HQ=4, HKV=2, D=64, q=[40, 70], ctx=[30, 0], W=5,
+                   at=[(0, 31, 0, 5), (0, 69, 1, 63), (1, 0, 0, 1), (1, 50, 1, 8)]),
+    "causal_128": dict(page=64, HQ=2, HKV=2, D=128, q=[150], ctx=[70], W=4,
+                       at=[(0, 75, 0, 127), (0, 130, 1, 64), (0, 200, 0, 0), (0, 219, 1, 33)]),
+    "window": dict(page=32, HQ=4, HKV=1, D=128, q=[90, 33], ctx=[200, 40], W=10, window=50, sinks=20,
+                   at=[(0, 18, 0, 3), (0, 100, 0, 4), (0, 160, 0, 77), (0, 230, 0, 100), (0, 289, 0, 9),
+                       (1, 10, 0, 11)]),
+    "pages_of_48": dict(page=48, HQ=2, HKV=1, D=64, q=[130], ctx=[20], W=4, at=[(0, 30, 0, 3), (0, 100, 0, 40)]),
+}
+
+
+@pytest.mark.parametrize("what", ["k", "v", "q"])
+@pytest.mark.parametrize("bound", [0, WIDE])
+@pytest.mark.parametrize("name", list(NANS))
+def test_prefill_keeps_a_nan_to_the_rows_that_see_it(dev, name, bound, what):
+    """A stored NaN reaches the rows that see its key, in V its own dim only; a
+    query's NaN its own row."""
+    c = dict(NANS[name], kv=E4M3)
+    g = torch.Generator().manual_seed(181)
+
+    def spoil(table, kc, vc, ks, vs):
+        for r, j, h, d in c["at"]:
+            if what != "q":
+                (kc if what == "k" else vc).view(torch.int8)[table[r][j // c["page"]], j % c["page"], h, d] = -1
+
+    q = None
+    if what == "q":
+        q = torch.randn(sum(c["q"]), c["HQ"], c["D"], generator=g).to(BF)
+        q[7, 1, 3], q[-1, 0] = math.nan, math.nan
+    got, lse, ref = _prefill(dev, c, g, bound, spoil, q)
+    _check_nan(got, lse, ref, (name, bound, what))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_keeps_a_nan_to_the_rows_that_see_it(dev, D):
+    from srswa import cache8
+    c = dict(page=16, HQ=6, HKV=2, D=D, W=160, kv=E4M3)
+    g = torch.Generator().manual_seed(191)
+    lens, dql = [2503, 61, 9], 5
+    table, kc, vc, ks, vs = _state(c, g, lens)
+    for r, j, h, d in ((0, 2500, 0, 3), (0, 2502, 1, 40), (1, 58, 0, 63), (2, 6, 1, 0), (2, 0, 0, 17)):
+        vc.view(torch.int8)[table[r][j // 16], j % 16, h, d] = 127
+    q = torch.randn(3 * dql, 6, D, generator=g).to(BF)
+    for win in (None, 7):
+        ref = O.attend(q, kc, vc, ks, vs, table, [0, 5, 10, 15], lens, 0.125, window=win, sinks=2)
+        got = cache8.cache8_decode(*(t.to(dev) for t in (q, kc, vc, ks, vs)),
+                                   torch.tensor(table, dtype=torch.int32).to(dev), torch.tensor(lens).to(dev),
+                                   scale=0.125, decode_query_len=dql, window=win, sinks=2, return_lse=True)
+        _check_nan(*got, ref, win)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_the_smallest_and_largest_v_scales(dev, dtype):
+    """A cache of zeros (scale 2^-100) and, in bf16, the largest finite values."""
+    from srswa import cache8
+    g = torch.Generator().manual_seed(201)
+    table, n = _table(g, [600, 600], 16, 38)
+    kc, ks = _cache(g, n, 16, 1, 64, E4M3)
+    vc, vs = _cache(g, n, 16, 1, 64, E4M3)
+    for p in table[0]:
+        vc.view(torch.int8)[p], vs[p] = 0, 2.0 ** -100
+    for p in table[1]:
+        vs[p] = 2.0 ** 119 if dtype == BF else 2.0 ** 4
+    q = torch.randn(2, 2, 64, generator=g).to(dtype)
+    ref = O.attend(q, kc, vc, ks, vs, table, [0, 1, 2], [600, 600], 0.125)
+    args = [t.to(dev) for t in (q, kc, vc, ks, vs)] + [torch.tensor(table, dtype=torch.int32).to(dev)]
+    lens = torch.tensor([600, 600]).to(dev)
+    _check(*cache8.cache8_decode(*args, lens, scale=0.125, return_lse=True), ref, "decode")
+    _check(*cache8.cache8_prefill(*args, torch.arange(3).to(dev), lens, WIDE, scale=0.125, return_lse=True), ref,
+           "tiles")
+
+
+def test_decode_and_append_of_many_requests(dev):
+    """More requests than a wave has lanes, long and short, shared out by units."""
+    from srswa import cache8
+    g = torch.Generator().manual_seed(211)
+    lens = torch.randint(0, 40, (130,), generator=g).tolist()
+    lens[3], lens[100], lens[129] = 5000, 3000, 4500
+    table, n = _table(g, [x + 30 for x in lens], 32, 160)
+    kc, ks = _cache(g, n, 32, 3, 64, torch.int8)
+    vc, vs = _cache(g, n, 32, 3, 64, torch.int8)
+    runs = torch.randint(0, 4, (130,), generator=g).tolist()
+    runs[66], runs[129] = 29, 30
+    k, v = (torch.randn(sum(runs), 3, 64, generator=g).to(BF) for _ in range(2))
+    ref = [O.append(x, y, s, table, lens, runs) for x, y, s in ((k, kc, ks), (v, vc, vs))]
+    d = [t.to(dev) for t in (k, v, kc, vc, ks, vs)]
+    bt = torch.tensor(table, dtype=torch.int32).to(dev)
+    cache8.cache8_append(*d, bt, torch.tensor(lens).to(dev),
+                         cu_seqlens=torch.tensor([0] + runs).cumsum(0).to(dev), max_new_len=30)
+    for got, want in zip(d[2:], (ref[0][0], ref[1][0], ref[0][1], ref[1][1])):
+        assert torch.equal(got.cpu(), want)
+    lens = [a + b for a, b in zip(lens, runs)]
+    q = torch.randn(130, 3, 64, generator=g).to(BF)
+    want = O.attend(q, ref[0][0], ref[1][0], ref[0][1], ref[1][1], table, list(range(131)), lens, 0.125)
+    _check(*cache8.cache8_decode(q.to(dev), *d[2:], bt, torch.tensor(lens).to(dev), scale=0.125, return_lse=True), want,
+           "130 requests")
+
+
+def test_many_selected_blocks_of_few_long_requests(dev):
+    """A table of selected blocks longer than the sequence has, shared out by units."""
+    from srswa.unlimited_dash_ops import dash_sparse_attn_decode
+    g = torch.Generator().manual_seed(221)
+    c = dict(page=16, HKV=2, D=128, W=320, kv=E4M3)
+    lens = [5000, 2000]
+    table, kc, vc, ks, vs = _state(c, g, lens)
+    ids = torch.stack([torch.randperm(330, generator=g)[:300] for _ in range(4)]).reshape(2, 2, 300).to(torch.int32)
+    q = torch.randn(2, 4, 128, generator=g).to(HF)
+    ref = O.attend(q, kc, vc, ks, vs, table, [0, 1, 2], lens, 0.1, window=32, topk=ids)
+    out = torch.empty_like(q, device=dev)
+    dash_sparse_attn_decode(q.to(dev), kc.to(dev), vc.to(dev), ids.to(dev), None,
+                            torch.tensor(table, dtype=torch.int32).to(dev), torch.tensor(lens).to(dev), 2, 0.1, out, 1,
+                            local_blocks=2, sparse_block_size=16, k_scale=ks.to(dev), v_scale=vs.to(dev))
+    _check(out, None, ref, "selected")
+
+
 # ------------------------------------------------------------ used together
 def _serve(dev, g, kv):
     """A pool, its caches and helpers for the runs below."""

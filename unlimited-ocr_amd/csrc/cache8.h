@@ -61,6 +61,23 @@ __device__ __forceinline__ void from_bytes4(uint32_t w, float* f) {
   }
 }
 
+// 0x80 in each byte of four that holds an e4m3 NaN (0x7f or 0xff)
+__device__ __forceinline__ uint32_t nan_bytes4(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// w with those bytes zeroed
+__device__ __forceinline__ uint32_t without(uint32_t w, uint32_t nan) { return w & ~((nan >> 7) * 0xffu); }
+
+// The sum l holds p' 2^-kLift / vs: between 2^-125 (one key, the largest bf16 value's
+// scale 2^120) and 2^127 (2^24 keys at the smallest scale, p' = 2^15) it stays a
+// normal number.
+constexpr int kLift = 12;
+
+// out = O inv_sum(M, L), lse = lse_of(M, L): M is -inf where no key was seen (L = 0)
+// and where every logit was NaN (L too).
+__device__ __forceinline__ float inv_sum(float M, float L) { return M == -INFINITY ? 0.f : 0x1p-12f / L; }
+__device__ __forceinline__ float lse_of(float M, float L) {
+  return M == -INFINITY ? L - INFINITY : (M + (log2f(L) + kLift)) * kLn2;
+}
+
 // A wave-uniform condition in a form the compiler must take for a lane's own, so
 // that the rare updates under it happen in place: under a uniform branch it copied
 // the whole set of accumulators to other registers on the common path.

@@ -183,6 +183,18 @@ __device__ __forceinline__ float xor16_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Four or eight e4m3 bytes of V: those that are NaN, and the bytes without them.
+__device__ __forceinline__ uint32_t nan_of(uint32_t v) { return nan_bytes4(v); }
+__device__ __forceinline__ uint32_t nan_of(uint2 v) { return nan_bytes4(v.x) | nan_bytes4(v.y); }
+__device__ __forceinline__ bool is_nan(uint32_t v, int d) { return (nan_bytes4(v) >> (8 * d + 7)) & 1u; }
+__device__ __forceinline__ bool is_nan(uint2 v, int d) { return is_nan(d < 4 ? v.x : v.y, d % 4); }
+__device__ __forceinline__ uint32_t without_nan(uint32_t v) { return without(v, nan_bytes4(v)); }
+__device__ __forceinline__ uint2 without_nan(uint2 v) { return make_uint2(without_nan(v.x), without_nan(v.y)); }
+__device__ __forceinline__ uint32_t shfl_bytes(uint32_t v, int l) { return __shfl(v, l, kWave); }
+__device__ __forceinline__ uint2 shfl_bytes(uint2 v, int l) {
+  return make_uint2(__shfl(v.x, l, kWave), __shfl(v.y, l, kWave));
+}
+
 // One unit's K and V bytes of a lane.
 template <int D>
 struct UnitBytes {
@@ -193,7 +205,8 @@ struct UnitBytes {
 
 // Item rows' attention over units [u_lo, u_end) of theirs: to out and lse, or to a
 // record (unnormalised, with m and l) where rec is not null.
-template <typename T, int KV, int D, bool SEL, int NW>
+// (MIX: a tile's rows may be of several tokens and V may hold NaN.)
+template <typename T, int KV, int D, bool SEL, bool MIX, int NW>
 __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile& t, int u_lo, int u_end, float* rec) {
   constexpr int NT = NW * kWave;
   constexpr int NL = D / 64;      // K loads per group
@@ -284,7 +297,7 @@ __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile&
       dvo[e] = (uint64_t)pg * (uint32_t)a.v_sp + (uint64_t)rw * (uint32_t)a.v_st;
       dks[e] = ok ? p.scale_l2 * a.k_scale[(int64_t)page * a.ks_sp + (int64_t)h * a.ks_sh] : 0.f;
       const float vs = ok ? fmaxf(a.v_scale[(int64_t)page * a.vs_sp + (int64_t)h * a.vs_sh], kScaleMin) : 1.f;
-      dvi[e] = 1.f / vs;
+      dvi[e] = 0x1p-12f / vs;                    // (kLift)
       db[e] += __log2f(vs);
       const int last = key + kGroup - 1;
       if constexpr (SEL)
@@ -378,6 +391,32 @@ __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile&
             }
           }
         }
+        if constexpr (MIX) {
+          // a NaN of a key that only some of the rows see is set in their O here, and
+          // is a zero in the products
+          uint32_t nan = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) nan |= nan_of(b.v[j]);
+          if (__any(nan != 0u)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int key = __builtin_amdgcn_readlane(dk[j / 4], i) + j % 4;
+#pragma unroll 1
+              for (int kg = 0; kg < 4; ++kg) {
+                const VB w = shfl_bytes(b.v[j], 16 * kg + n);      // key `key + 4 kg`, this lane's dims of O
+                if (!__any(nan_of(w) != 0u)) continue;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const int pos = t.p0 + (t.row0 + 4 * g + x) / p.G, k = key + 4 * kg;
+                  const bool see = (k <= pos) & ((a.window == 0) | (k > pos - a.window) | (k < a.sinks));
+#pragma unroll
+                  for (int d = 0; d < DV; ++d) acc[d][x] = (see & is_nan(w, d)) ? NAN : acc[d][x];
+                }
+              }
+              b.v[j] = without_nan(b.v[j]);
+            }
+          }
+        }
       }
       float zm = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
       if (per_lane(__any(zm > thr))) {
@@ -463,15 +502,14 @@ __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile&
     }
     if (!rec) {
       const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
-      const float inv = M == -INFINITY ? 0.f : 1.f / L;
+      const float inv = inv_sum(M, L);
       T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn + (int64_t)ho * a.o_sh + c;
       uint2 w;
       w.x = Mfma<T>::pack2(o.x * inv, o.y * inv);
       w.y = Mfma<T>::pack2(o.z * inv, o.w * inv);
       *reinterpret_cast<uint2*>(op) = w;
       if (a.lse && c == 0)
-        a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] =
-            M == -INFINITY ? -INFINITY : (M + log2f(L)) * kLn2;
+        a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] = lse_of(M, L);
     } else {
       *reinterpret_cast<float4*>(rec + rr * D + c) = o;
       if (c == 0) {
@@ -487,7 +525,7 @@ __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile&
 // side, on neighbouring XCDs: their rows share DRAM pages (a share's heads on one
 // XCD 305 us, one head's shares first 340 us against 261 us, 48 requests of 700 to
 // 40,000 keys, ten heads).
-template <typename T, int KV, int D, bool SEL, int NW>
+template <typename T, int KV, int D, bool SEL, bool MIX, int NW>
 __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3))) void cache8_decode_kernel(AttendK p) {
   const srswa_cache8_attend_args& a = p.a;
   const int lane = threadIdx.x % kWave;
@@ -504,7 +542,7 @@ __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
   }
   if (p.shares == 0) {
     const Tile t = tile_of<SEL>(p, id / p.tiles, id % p.tiles);
-    if (t.nrows > 0) attend_item<T, KV, D, SEL, NW>(p, h, t, 0, t.units, nullptr);
+    if (t.nrows > 0) attend_item<T, KV, D, SEL, MIX, NW>(p, h, t, 0, t.units, nullptr);
     return;
   }
   Share sh;
@@ -519,7 +557,7 @@ __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
     const int64_t end = start + max(t.units, 1);
     const bool whole = s == start && e >= end;
     if (!first) __syncthreads();                 // the item before is written from LDS
-    attend_item<T, KV, D, SEL, NW>(p, h, t, (int)(s - start), (int)min((int64_t)t.units, min(e, end) - start),
+    attend_item<T, KV, D, SEL, MIX, NW>(p, h, t, (int)(s - start), (int)min((int64_t)t.units, min(e, end) - start),
                                    whole ? nullptr : recs + (first ? 0 : p.rs * (D + 2)));
     first = false;
     s = start = end;
@@ -580,7 +618,7 @@ __global__ __launch_bounds__(kWave) void cache8_merge_kernel(AttendK p) {
     }
   }
   const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
-  const float inv = M == -INFINITY ? 0.f : 1.f / L;
+  const float inv = inv_sum(M, L);
   T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn + (int64_t)ho * a.o_sh + DL * lane;
   if constexpr (DL == 2) {
     *reinterpret_cast<uint32_t*>(op) = Mfma<T>::pack2(o[0] * inv, o[1] * inv);
@@ -588,8 +626,7 @@ __global__ __launch_bounds__(kWave) void cache8_merge_kernel(AttendK p) {
     *reinterpret_cast<uint16_t*>(op) = (uint16_t)(Mfma<T>::pack2(o[0] * inv, 0.f) & 0xffffu);
   }
   if (a.lse && lane == 0)
-    a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] =
-        M == -INFINITY ? -INFINITY : (M + log2f(L)) * kLn2;
+    a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] = lse_of(M, L);
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -665,13 +702,14 @@ AttendK plan(const srswa_cache8_attend_args* a) {
   p.scale_l2 = a->scale * kLog2e;
   const int64_t rows = (int64_t)a->max_query_len * p.G;
   p.tiles = (int)(a->topk ? (int64_t)a->max_query_len * ((p.G + kRows - 1) / kRows) : (rows + kRows - 1) / kRows);
-  p.items = a->R * p.tiles;
+  const int64_t items = (int64_t)a->R * p.tiles;
+  p.items = (int)std::min<int64_t>(items, INT32_MAX);
   p.rs = (int)std::min<int64_t>(kRows, a->topk ? p.G : rows);
   int64_t groups = (int64_t)a->max_blocks * a->page_size / kGroup;
   if (a->topk) groups = (int64_t)a->topk_n * p.gpp + std::min<int64_t>(groups, a->window / kGroup + 2);
   else if (a->window > 0)
     groups = std::min<int64_t>(groups, ((int64_t)a->window + a->max_query_len) / kGroup + 2 + (a->sinks + kGroup - 1) / kGroup);
-  const int64_t units = (groups + 1) / 2, wgs = (int64_t)p.items * a->HKV;
+  const int64_t units = (groups + 1) / 2, wgs = items * a->HKV;
   p.most_units = units;
   p.pairs = a->D == 64 && a->HKV % 2 == 0;
   int cus = device_cu_count();
@@ -687,7 +725,11 @@ size_t ws_bytes_of(const AttendK& p) {
 
 template <typename T, int KV, int D, bool SEL>
 void launch(const AttendK& p, unsigned grid, hipStream_t st) {
-  cache8_decode_kernel<T, KV, D, SEL, 4><<<grid, 4 * kWave, 0, st>>>(p);
+  // (the code that a NaN of a key which not every row sees takes costs 48 uneven
+  // single-token requests 5%)
+  constexpr bool kMix = KV == kFp8E4M3FN && !SEL;
+  if (kMix && p.a.max_query_len > 1) cache8_decode_kernel<T, KV, D, SEL, kMix, 4><<<grid, 4 * kWave, 0, st>>>(p);
+  else cache8_decode_kernel<T, KV, D, SEL, false, 4><<<grid, 4 * kWave, 0, st>>>(p);
   if (p.shares > 0)
     cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.items * p.a.HKV * p.rs), kWave, 0, st>>>(p);
 }
@@ -733,7 +775,7 @@ size_t cache8_decode_ws(const srswa_cache8_attend_args* a) { return ws_bytes_of(
 
 void cache8_decode_load(const srswa_cache8_attend_args* a, int64_t* wgs, int64_t* units) {
   const AttendK p = plan(a);
-  *wgs = (int64_t)p.items * a->HKV;
+  *wgs = (int64_t)a->R * p.tiles * a->HKV;
   *units = p.most_units;
 }
 

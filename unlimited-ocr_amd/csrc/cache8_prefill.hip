@@ -33,12 +33,12 @@ constexpr float kBelow = 7.f, kSlack = 8.f;
 
 struct PrefillK {
   srswa_cache8_attend_args a;
-  int G, tiles, nsplit, groups;   // groups = R * HKV * nsplit
+  int G, tiles, nsplit;           // tiles: of all requests at most
   uint32_t page_mul;              // key / page_size = umulhi(key, page_mul) >> page_shift
   int page_shift;
   float scale_l2;
   bool by_group;                  // the tiles of a group to one XCD, else in turn
-  float* part;                    // [R * HKV * tiles][nsplit][128 * (D + 2)]
+  float* part;                    // [tiles][HKV][nsplit][128 * (D + 2)]
 };
 
 template <int D> struct Lds {
@@ -76,12 +76,6 @@ __device__ __forceinline__ Tile tile_of(const PrefillK& p, int r, int tile) {
   t.c1 = max(lo / kChunk, t.c0);
   t.chunks = t.c0 + max((t.end + kChunk - 1) / kChunk - t.c1, 0);
   return t;
-}
-
-// c + the sum of a packed fp16 pair
-__device__ __forceinline__ float dot2_ones(uint32_t w, float c) {
-  const f16x2_native_t one = {(_Float16)1.f, (_Float16)1.f};
-  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_native_t, w), one, c, false);
 }
 
 // Tile number b over all requests' own tiles: its request and place there, the
@@ -137,11 +131,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   // longer ones first.  Several: workgroups count only the tiles that the requests
   // have, so every XCD gets as many to one (six requests of 70 to 1,900 rows, ten
   // heads, 500 tiles for 512 places: 81 -> 58 us against tiles up to the longest).
-  int r, tile, h, part;
+  int r, tile, nth, h, part;
   if (p.by_group) {
     const int gi = (int)(blockIdx.x % kXcds) + kXcds * (int)(blockIdx.x / kXcds / p.tiles);
-    if (gi >= p.groups) return;
-    tile = p.tiles - 1 - (int)(blockIdx.x / kXcds % p.tiles);
+    if (gi >= a.HKV * p.nsplit) return;
+    tile = nth = p.tiles - 1 - (int)(blockIdx.x / kXcds % p.tiles);
     part = gi % p.nsplit;
     h = gi / p.nsplit;
     r = 0;
@@ -149,7 +143,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     const int b = (int)blockIdx.x / p.nsplit;
     part = (int)blockIdx.x % p.nsplit;
     h = b % a.HKV;
-    if (!nth_tile(p, b / a.HKV, lane, &r, &tile)) return;
+    nth = b / a.HKV;
+    if (!nth_tile(p, nth, lane, &r, &tile)) return;
   }
   const Tile t = tile_of(p, r, tile);
   if (t.nrows == 0) return;
@@ -232,6 +227,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       f.vb[i] = *reinterpret_cast<const uint2*>(vp + voff);
     }
   };
+  // rows at positions lo .. hi each see every key of the chunk at j
+  auto seen_whole = [&](int j, int lo, int hi) __attribute__((always_inline)) {
+    return j + kChunk - 1 <= lo && j + kChunk <= t.kend && (a.window == 0 || j > hi - a.window || j + kChunk <= a.sinks);
+  };
+  uint32_t nans = 0;                 // not 0: this thread met such a NaN
   auto stage = [&](int u, int buf, Fetched& f) __attribute__((always_inline)) {
     const int j = base_of(u);
     const bool ok = f.page >= 0 && f.page < a.num_pages && j + lq * kGroup < t.end;
@@ -250,6 +250,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         f.vb[i].y = any ? f.vb[i].y : 0u;
       }
     }
+    if constexpr (KV == kFp8E4M3FN) {
+      // a NaN of a key that only some rows see is a zero in the products and is set
+      // in their O after the loop
+      if (per_lane(!seen_whole(j, t.pmin, t.pmax))) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const uint32_t nx = nan_bytes4(f.vb[i].x), ny = nan_bytes4(f.vb[i].y);
+          nans |= nx | ny;
+          f.vb[i].x = without(f.vb[i].x, nx);
+          f.vb[i].y = without(f.vb[i].y, ny);
+        }
+      }
+    }
     uint16_t* sK = reinterpret_cast<uint16_t*>(smem + buf * L::buf) + srow * KP + scol;
     uint16_t* sV = reinterpret_cast<uint16_t*>(smem + buf * L::buf + L::kBytes) + srow * VP + scol;
 #pragma unroll
@@ -262,7 +275,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     if (tid < 4) {
       const float vs = ok ? fmaxf(f.gv, kScaleMin) : 1.f;
       reinterpret_cast<float4*>(smem + buf * L::buf + L::kBytes + L::vBytes)[tid] =
-          make_float4(ok ? f.gk * p.scale_l2 : 0.f, ok ? __log2f(vs) : -INFINITY, __builtin_amdgcn_rcpf(vs), 0.f);
+          make_float4(ok ? f.gk * p.scale_l2 : 0.f, ok ? __log2f(vs) : -INFINITY, 0x1p-12f * __builtin_amdgcn_rcpf(vs), 0.f);   // (kLift)
     }
   };
 
@@ -299,8 +312,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
       for (int q = 0; q < 4; ++q) gs[q] = sg[ONE ? 0 : q];
       // (a group without a page has K zero and an exponent of -inf, and needs no mask)
-      const bool whole = j0 + kChunk - 1 <= wpmin && j0 + kChunk <= t.kend &&
-                         (a.window == 0 || j0 > wpmax - a.window || j0 + kChunk <= a.sinks);
+      const bool whole = seen_whole(j0, wpmin, wpmax);
       f32x16_t s[2];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -356,7 +368,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           for (int j = 0; j < 8; ++j) pe[j] = __builtin_amdgcn_exp2f(s[kt][8 * q + j]);
           const uint4 pf = make_uint4(pack_f16(pe[0], pe[1]), pack_f16(pe[2], pe[3]), pack_f16(pe[4], pe[5]),
                                       pack_f16(pe[6], pe[7]));
-          sum = dot2_ones(pf.w, dot2_ones(pf.z, dot2_ones(pf.y, dot2_ones(pf.x, 0.f))));   // of the rounded weights
+          sum = ((pe[0] + pe[1]) + (pe[2] + pe[3])) + ((pe[4] + pe[5]) + (pe[6] + pe[7]));
           l = fmaf(sum, gs[2 * kt + q].z, l);
 #pragma unroll
           for (int d = 0; d < MT; ++d)
@@ -373,11 +385,37 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     if (u + 1 < u_hi) step(u + 1, 1, fb);
   }
 
+  if constexpr (KV == kFp8E4M3FN) {
+    int* met = reinterpret_cast<int*>(smem);               // (the last step's barrier is behind)
+    const bool any = __any(nans != 0u);
+    if (lane == 0) met[wave] = any;
+    __syncthreads();
+    if (met[0] | met[1] | met[2] | met[3]) {
+      for (int u = u_lo; u < u_hi; ++u) {
+        const int j = base_of(u);
+        if (seen_whole(j, t.pmin, t.pmax)) continue;
+        for (int k = j; k < min(j + kChunk, t.end); ++k) {
+          const int page = a.block_table[(int64_t)r * a.bt_sr + block_of(k)];
+          if (page < 0 || page >= a.num_pages) continue;
+          const bool see = ((uint32_t)(k - my_lo) < my_span) | ((uint32_t)k < my_first);
+          const uint8_t* vp = vcache + offset(page, a.v_sp) + offset(k - block_of(k) * a.page_size, a.v_st) + 4 * hh;
+#pragma unroll
+          for (int d = 0; d < MT; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const uint32_t n = see ? nan_bytes4(*reinterpret_cast<const uint32_t*>(vp + 32 * d + 8 * x)) : 0u;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][4 * x + e] = (n >> (8 * e + 7)) & 1u ? NAN : o[d][4 * x + e];
+            }
+        }
+      }
+    }
+  }
   l = xor32_sum(l);
   if (!wave_live) return;
   if (p.nsplit > 1 && parts > 1) {
     // record: lane-major float4s, then the rows' (m, l)
-    float* rec = p.part + (((int64_t)(r * a.HKV + h) * p.tiles + tile) * p.nsplit + part) * kRowsWg * (D + 2);
+    float* rec = p.part + (((int64_t)nth * a.HKV + h) * p.nsplit + part) * kRowsWg * (D + 2);
 #pragma unroll
     for (int d = 0; d < MT; ++d)
 #pragma unroll
@@ -391,7 +429,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     return;
   }
   if (wrow >= t.nrows) return;
-  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  const float inv = inv_sum(m, l);
   T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + tok) * a.o_sn + (int64_t)hq * a.o_sh + 4 * hh;
 #pragma unroll
   for (int d = 0; d < MT; ++d)
@@ -401,7 +439,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           make_uint2(Mfma<T>::pack2(o[d][4 * x] * inv, o[d][4 * x + 1] * inv),
                      Mfma<T>::pack2(o[d][4 * x + 2] * inv, o[d][4 * x + 3] * inv));
   if (a.lse && hh == 0)
-    a.lse[(int64_t)(t.q0 + tok) * a.lse_sn + (int64_t)hq * a.lse_sh] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+    a.lse[(int64_t)(t.q0 + tok) * a.lse_sn + (int64_t)hq * a.lse_sh] = lse_of(m, l);
 }
 
 // Joins the parts of a tile, lane by lane as they were written: one workgroup per
@@ -410,7 +448,9 @@ template <typename T, int D>
 __global__ __launch_bounds__(2 * D) void cache8_join_kernel(PrefillK p) {
   const srswa_cache8_attend_args& a = p.a;
   const int wave = (int)blockIdx.x % 4, rt = (int)blockIdx.x / 4;     // the wave that wrote the rows
-  const int tile = rt % p.tiles, rh = rt / p.tiles, h = rh % a.HKV, r = rh / a.HKV;
+  const int h = rt % a.HKV;
+  int r, tile;
+  if (!nth_tile(p, rt / a.HKV, (int)threadIdx.x % kWave, &r, &tile)) return;
   const Tile t = tile_of(p, r, tile);
   const int parts = parts_of(p, t);
   if (wave * 32 >= t.nrows || parts == 1) return;
@@ -437,14 +477,14 @@ __global__ __launch_bounds__(2 * D) void cache8_join_kernel(PrefillK p) {
   }
   if (wrow >= t.nrows) return;
   const int row = t.row0 + wrow, tok = row / p.G, hq = h * p.G + row % p.G;
-  const float inv = M == -INFINITY ? 0.f : 1.f / l;
+  const float inv = inv_sum(M, l);
   T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + tok) * a.o_sn + (int64_t)hq * a.o_sh + 32 * d + 4 * hh;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     *reinterpret_cast<uint2*>(op + 8 * i) = make_uint2(Mfma<T>::pack2(o[i].x * inv, o[i].y * inv),
                                                        Mfma<T>::pack2(o[i].z * inv, o[i].w * inv));
   if (a.lse && hh == 0 && d == 0)
-    a.lse[(int64_t)(t.q0 + tok) * a.lse_sn + (int64_t)hq * a.lse_sh] = M == -INFINITY ? -INFINITY : (M + log2f(l)) * kLn2;
+    a.lse[(int64_t)(t.q0 + tok) * a.lse_sn + (int64_t)hq * a.lse_sh] = lse_of(M, l);
 }
 
 // Parts: the fewest that need the least rounds of the GPU per part, where two
@@ -456,7 +496,9 @@ PrefillK plan(const srswa_cache8_attend_args* a) {
   p.a = *a;
   p.G = a->HQ / a->HKV;
   p.scale_l2 = a->scale * kLog2e;
-  p.tiles = (int)(((int64_t)a->max_query_len * p.G + kRowsWg - 1) / kRowsWg);
+  // as many tiles as the rows can make: the longest request may be shorter than its bound
+  p.tiles = (int)std::min<int64_t>((int64_t)a->R * (((int64_t)a->max_query_len * p.G + kRowsWg - 1) / kRowsWg),
+                                   (int64_t)a->total_q * p.G / kRowsWg + a->R);
   int lg = 0;
   while ((1 << lg) < a->page_size) ++lg;
   p.page_shift = lg - 1;
@@ -483,20 +525,19 @@ PrefillK plan(const srswa_cache8_attend_args* a) {
     }
   p.by_group = least[1] <= least[0] * 1.02;
   p.nsplit = parts[p.by_group];
-  p.groups = a->R * a->HKV * p.nsplit;
   return p;
 }
 
 size_t ws_bytes_of(const PrefillK& p) {
-  return p.nsplit > 1 ? (size_t)p.groups * p.tiles * kRowsWg * (p.a.D + 2) * sizeof(float) : 0;
+  return p.nsplit > 1 ? (size_t)p.tiles * p.a.HKV * p.nsplit * kRowsWg * (p.a.D + 2) * sizeof(float) : 0;
 }
 
 // Few rows per request, or little work in all, take decode's form of 16-row items: a
 // 128-row tile converts each key once for eight times the rows, but fills fewer CUs
-// and takes longer to start and to end.  One request of ten heads, 16-row items against tiles: 49 against
-// 68 us (32 rows after 30,720 keys), 104 against 75 (128 rows), 11.5 against 22
-// (512 rows, no prefix); eight requests: 24.6 against 35 (64 rows after up to 2,000
-// keys), 41 against 31 (512 rows, no prefix).
+// and takes longer to start and to end.  One request of ten heads, 16-row items
+// against tiles: 49 against 68 us (32 rows after 30,720 keys), 104 against 75 (128
+// rows), 11.5 against 22 (512 rows, no prefix); eight requests: 24.6 against 35 (64
+// rows after up to 2,000 keys), 41 against 31 (512 rows, no prefix).
 bool narrow(const srswa_cache8_attend_args* a) {
   if ((int64_t)a->max_query_len * (a->HQ / a->HKV) <= 32) return true;
   int64_t wgs, units;
@@ -519,7 +560,7 @@ int launch(const PrefillK& p, unsigned grid, hipStream_t st) {
                                              : launch_tiles<T, KV, D, false>(p, grid, st);
   if (rc != SRSWA_OK) return rc;
   if (p.nsplit > 1)
-    cache8_join_kernel<T, D><<<(unsigned)(p.a.R * p.a.HKV * p.tiles * 4), 2 * D, 0, st>>>(p);
+    cache8_join_kernel<T, D><<<(unsigned)(p.a.HKV * p.tiles * 4), 2 * D, 0, st>>>(p);
   return SRSWA_OK;
 }
 template <typename T, int KV>
@@ -562,10 +603,9 @@ extern "C" int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws,
     return SRSWA_WORKSPACE;
   }
   p.part = reinterpret_cast<float*>(ws);
-  // several requests: as many tiles as their rows can make
-  const int64_t own = std::min<int64_t>((int64_t)a->R * p.tiles, (int64_t)a->total_q * p.G / kRowsWg + a->R);
-  const int64_t grid = p.by_group ? ((int64_t)p.groups + kXcds - 1) / kXcds * kXcds * p.tiles : own * a->HKV * p.nsplit;
-  if (grid > 0x7fffffff || (int64_t)a->R * a->HKV * p.nsplit > 0x7fffffff) {
+  const int64_t parts = (int64_t)a->HKV * p.nsplit;
+  const int64_t grid = (p.by_group ? (parts + kXcds - 1) / kXcds * kXcds : parts) * p.tiles;
+  if (grid > 0x7fffffff || (int64_t)a->HKV * p.tiles * 4 > 0x7fffffff) {
     set_error("%s: grid too large", what);
     return SRSWA_UNSUPPORTED;
   }

@@ -186,7 +186,8 @@ def cache8_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, 
     decode_query_len + t and sees the keys j <= p, with a window only j > p -
     window and the first ``sinks`` keys.  Returns out [rows, HQ, D] in q's dtype
     (0 for a row that sees no key) and, if asked, lse [rows, HQ] (natural log,
-    -inf there).  A stored NaN reaches the rows of its request only."""
+    -inf there).  A stored NaN reaches the rows that see its key, in V its own dim
+    only."""
     w, s = _window(window, sinks)
     if _lib.host:
         got = _lib.host.attend(0, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, None, decode_query_len,
