@@ -587,6 +587,45 @@ def test_decode_and_append_of_many_requests(dev):
            "130 requests")
 
 
+def test_offsets_past_32_bits(dev):
+    """Pages more than 2^32 bytes into a cache: append, decode, prefill and a page copy there."""
+    from srswa import cache8, cache_pages
+    g = torch.Generator().manual_seed(231)
+    page, H, D, N = 64, 4, 128, 140_000
+    far = torch.zeros(2, N, page, H, D, dtype=torch.int8, device=dev)
+    sc = torch.ones(2, N, H, device=dev)
+    lens, ids = [150, 70], [N - 1, 7, N - 3, N - 9, 131_073]
+    kc, ks = _cache(g, 6, page, H, D, torch.int8)
+    vc, vs = _cache(g, 6, page, H, D, torch.int8)
+    table = [[0, 1, 2], [3, 4, -1]]
+    far_table = torch.tensor([[ids[x] if x >= 0 else -1 for x in row] for row in table], dtype=torch.int32).to(dev)
+    for i, x in enumerate(ids):
+        far[0, x], far[1, x], sc[0, x], sc[1, x] = kc[i].to(dev), vc[i].to(dev), ks[i].to(dev), vs[i].to(dev)
+    k, v = (torch.randn(2, H, D, generator=g).to(BF) for _ in range(2))
+    kc, ks = O.append(k, kc, ks, table, lens, [1, 1])
+    vc, vs = O.append(v, vc, vs, table, lens, [1, 1])
+    state = (far[0], far[1], sc[0], sc[1])
+    sl = torch.tensor(lens, dtype=torch.int32).to(dev)
+    cache8.cache8_append(k.to(dev), v.to(dev), *state, far_table, sl)
+    lens, sl = [n + 1 for n in lens], sl + 1
+    q = torch.randn(2 * 40, H, D, generator=g).to(BF)
+    ref = O.attend(q, kc, vc, ks, vs, table, [0, 40, 80], lens, 0.1)
+    for bound in (40, WIDE):
+        got = cache8.cache8_prefill(q.to(dev), *state, far_table, torch.tensor([0, 40, 80]).to(dev), sl, bound, scale=0.1,
+                                    return_lse=True)
+        _check(*got, ref, bound)
+    pool = torch.zeros(N, dtype=torch.int32, device=dev)
+    pool[far_table[far_table >= 0].long()] = 1
+    pool[:N - 2] += 1                                     # held by others: the free page is the last but one
+    pool[N - 2] = 0
+    st, missing = cache_pages.pages_reorder(cache_pages.PageTable(far_table, sl, pool), torch.zeros_like(sl), state,
+                                            page_size=page)
+    assert int(missing) == 0 and st.block_table[1].tolist() == [N - 1, 7, N - 2]
+    o, lse = cache8.cache8_decode(q[38:40].to(dev), *state, st.block_table, st.seq_lens, scale=0.1, return_lse=True)
+    one = O.attend(q[38:40], kc, vc, ks, vs, [table[0], table[0]], [0, 1, 2], [lens[0]] * 2, 0.1)
+    _check(o, lse, one, "forked")
+
+
 def test_many_selected_blocks_of_few_long_requests(dev):
     """A table of selected blocks longer than the sequence has, shared out by units."""
     from srswa.unlimited_dash_ops import dash_sparse_attn_decode

@@ -203,3 +203,19 @@ def test_abi_refuses_before_any_launch():
         assert L.srswa_cache8_decode(ctypes.byref(a), None, 0, None) == _lib.SRSWA_OK
     b = _lib.Cache8AppendArgs()
     assert L.srswa_cache8_append(ctypes.byref(b), None) == I
+
+
+def test_abi_refuses_far_strides_and_large_grids():
+    """Strides that 32-bit address parts cannot hold, and launches past the grid."""
+    L = _lib.lib()
+    U = _lib.SRSWA_UNSUPPORTED
+    for over in (dict(k_sp=1 << 31), dict(v_sp=(1 << 31) + 16), dict(k_st=1 << 31), dict(v_sh=1 << 31), dict(k_sp=-16),
+                 dict(ks_sp=1 << 31), dict(vs_sp=-1)):
+        a = _attend_struct(**over)
+        for fn in (L.srswa_cache8_decode, L.srswa_cache8_prefill):
+            assert fn(ctypes.byref(a), None, 0, None) == U, over
+    a = _attend_struct(R=1 << 15, total_q=1 << 15, HQ=1 << 18, HKV=1 << 18, q_sn=1 << 24, o_sn=1 << 24)
+    assert L.srswa_cache8_decode(ctypes.byref(a), None, 0, None) == U
+    # a bound on the longest request that no table of items could hold: sized by the rows there are
+    a = _attend_struct(R=4096, total_q=4096, max_query_len=1 << 30, cu_seqlens_q=0x900000)
+    assert L.srswa_cache8_prefill_workspace(ctypes.byref(a)) < 1 << 32

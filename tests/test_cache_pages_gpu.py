@@ -120,6 +120,58 @@ def test_compact(dev, R, W, N, page):
         _equal(state, table, lens, ref)
 
 
+# rows and entries past a workgroup's width, pages past its tiles, tables past the one-workgroup plan
+@pytest.mark.parametrize("R,W,N,page", [(1500, 3, 2500, 16), (300, 400, 9000, 16), (5, 8000, 36000, 16),
+                                        (3, 300, 600000, 32)])
+def test_larger_pools(dev, R, W, N, page):
+    from srswa import cache_pages
+    table, lens, ref, g = _pool(90, R, W, N, page, share=5)
+    data = torch.randn(N, 3, generator=g)
+    d = [data.to(dev)]
+    state = _dev(dev, table, lens, ref)
+    new = [min(n + 3 * page * (i % 4), W * page) for i, n in enumerate(lens)]
+    st, missing = cache_pages.pages_reserve(state, torch.tensor(new).to(dev), page_size=page)
+    table, ref, m = O.reserve(table, ref, new, page)
+    _equal(st, table, new, ref)
+    assert missing.tolist() == [m]
+    par = torch.randint(-1, R, (R,), generator=g).tolist()
+    st, missing = cache_pages.pages_reorder(st, torch.tensor(par).to(dev), d, page_size=page)
+    table, lens, ref, m, copies = O.reorder(table, new, ref, par, page)
+    _equal(st, table, lens, ref)
+    assert missing.tolist() == [m]
+    for s, e in copies:
+        data[e] = data[s]
+    st, live = cache_pages.pages_compact(st, d)
+    table, ref, n, moves = O.compact(table, ref)
+    _equal(st, table, lens, ref)
+    assert live.tolist() == [n]
+    for s, e in moves:
+        data[e] = data[s]
+    assert torch.equal(d[0].cpu(), data)
+
+
+def test_pages_on_other_streams_at_once(dev):
+    """The same state reordered on two streams, each with its own caches."""
+    from srswa import cache_pages
+    table, lens, ref, g = _pool(95, 40, 20, 700, 16)
+    par = torch.randint(-1, 40, (40,), generator=g)
+    t, ln, rf, m, copies = O.reorder(table, lens, ref, par.tolist(), 16)
+    state, par = _dev(dev, table, lens, ref), par.to(torch.int32).to(dev)
+    data = torch.randn(700, 2048, generator=g)
+    d = [data.to(dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(2):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.append(cache_pages.pages_reorder(state, par, [d[i]], page_size=16))
+    torch.cuda.synchronize()
+    for s, e in copies:
+        data[e] = data[s]
+    for (st, missing), x in zip(got, d):
+        _equal(st, t, ln, rf)
+        assert missing.tolist() == [m] and torch.equal(x.cpu(), data)
+
+
 def test_out_and_many_caches(dev):
     """More caches than one copy launch takes, and states written in turn."""
     from srswa import cache_pages

@@ -132,7 +132,8 @@ def pages_reorder(state, parents, caches, *, page_size, out=None):
     one gets a copy of the page the parent has begun, in every cache.  Pages
     nobody holds any more become free and may be dealt in the same call.
     Returns (state, missing): ``missing`` counts copies that found no free page
-    (that entry is -1)."""
+    (that entry is -1).  A shared page stays shared: a row's ``seq_lens`` must not
+    be set back into one."""
     return _run("reorder", state, parents, tuple(caches), page_size, out)
 
 
