@@ -626,6 +626,29 @@ def test_offsets_past_32_bits(dev):
     _check(o, lse, one, "forked")
 
 
+def test_a_page_s_rows_far_apart(dev):
+    """A cache stored by place in the page first: token strides past 2^25 bytes."""
+    from srswa import cache8
+    g = torch.Generator().manual_seed(241)
+    page, H, D, N = 64, 4, 128, 65_700
+    base = torch.zeros(page, N, H, D, dtype=torch.int8, device=dev)
+    far = base.permute(1, 0, 2, 3)
+    assert far.stride(1) > 1 << 25
+    lens, table, ids = [150, 64], [[0, 1, 2], [3, -1, -1]], [N - 1, 7, N - 3, 40_000]
+    kc, ks = _cache(g, 4, page, H, D, torch.int8)
+    _, vs = _cache(g, 4, page, H, D, torch.int8)
+    sk, sv = torch.ones(N, H, device=dev), torch.ones(N, H, device=dev)
+    for i, x in enumerate(ids):
+        far[x], sk[x], sv[x] = kc[i].to(dev), ks[i].to(dev), vs[i].to(dev)
+    bt = torch.tensor([[ids[x] if x >= 0 else -1 for x in row] for row in table], dtype=torch.int32).to(dev)
+    q = torch.randn(80, H, D, generator=g).to(BF)
+    ref = O.attend(q, kc, kc, ks, vs, table, [0, 40, 80], lens, 0.1)
+    for bound in (40, WIDE):
+        got = cache8.cache8_prefill(q.to(dev), far, far, sk, sv, bt, torch.tensor([0, 40, 80]).to(dev),
+                                    torch.tensor(lens).to(dev), bound, scale=0.1, return_lse=True)
+        _check(*got, ref, bound)
+
+
 def test_many_selected_blocks_of_few_long_requests(dev):
     """A table of selected blocks longer than the sequence has, shared out by units."""
     from srswa.unlimited_dash_ops import dash_sparse_attn_decode

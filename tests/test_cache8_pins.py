@@ -209,7 +209,7 @@ def test_abi_refuses_far_strides_and_large_grids():
     """Strides that 32-bit address parts cannot hold, and launches past the grid."""
     L = _lib.lib()
     U = _lib.SRSWA_UNSUPPORTED
-    for over in (dict(k_sp=1 << 31), dict(v_sp=(1 << 31) + 16), dict(k_st=1 << 31), dict(v_sh=1 << 31), dict(k_sp=-16),
+    for over in (dict(k_sp=1 << 31), dict(v_sp=(1 << 31) + 16), dict(k_st=1 << 28), dict(v_st=1 << 31), dict(v_sh=1 << 31), dict(k_sp=-16),
                  dict(ks_sp=1 << 31), dict(vs_sp=-1)):
         a = _attend_struct(**over)
         for fn in (L.srswa_cache8_decode, L.srswa_cache8_prefill):

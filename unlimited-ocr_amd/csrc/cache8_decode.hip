@@ -672,6 +672,10 @@ int cache8_check(const srswa_cache8_attend_args* a, const char* what) {
       set_error("%s: cache strides must keep rows 16-byte aligned and be below 2^31", what);
       return SRSWA_UNSUPPORTED;
     }
+  if (a->k_st >= 1 << 28 || a->v_st >= 1 << 28) {     // (16 rows of a group lie within 2^32 bytes)
+    set_error("%s: token strides must be below 2^28", what);
+    return SRSWA_UNSUPPORTED;
+  }
   if (a->ks_sp < 0 || a->ks_sp > INT32_MAX || a->vs_sp < 0 || a->vs_sp > INT32_MAX) {
     set_error("%s: scale strides must be below 2^31", what);
     return SRSWA_UNSUPPORTED;

@@ -4,17 +4,16 @@
 // One workgroup = (request, kv head, tile of 128 rows, part of its keys): four
 // waves of 32 rows, a row being a (token, query head of the group) pair, two
 // workgroups per CU.  Per chunk of 64 keys:
-//   * the chunk's bytes, fetched into registers three chunks ahead, are converted
-//     once for all four waves and stored to LDS, K in q's type and V in fp16
-//     (both exact), into the buffer that the previous chunk does not use: one
-//     barrier per chunk;
+//   * the next chunk's bytes, fetched into registers one chunk before, are
+//     converted once for all four waves and stored to the other LDS buffer, K in
+//     q's type and V in fp16 (both exact), beside the products K Q^T: one barrier
+//     per chunk;
 //   * S^T = K Q^T on v_mfma_f32_32x32x16: every lane owns one row and 32 keys;
 //   * a 16-key group lies in one page, so its scales are uniform: z' = scale ks s
 //     + log2 vs - m in one FMA, p' = 2^z' weighs V's bytes, l += p' / vs (see
 //     cache8_decode.hip for the range of p');
 //   * O^T += V^T P^T in fp16, V^T read by ds_read_b64_tr_b16.
-// A chunk that every row of a wave sees whole takes no mask; one that none sees
-// is skipped by the wave.  Parts (few tiles, long keys) write fp32 records that
+// A chunk that every row of a wave sees whole takes no mask.  Parts (few tiles, long keys) write fp32 records that
 // cache8_join_kernel combines.
 #include <algorithm>
 
@@ -177,8 +176,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   // zeroed as it is stored, for 0 * NaN would reach O.
   const int srow = tid / PPR, scol = tid % PPR * 8;
   const int wgrp = wave * kWave / PPR / kGroup;                     // the wave's group in pass 0
-  const uint32_t koff = (uint32_t)(srow - wgrp * kGroup) * (uint32_t)a.k_st + scol;
-  const uint32_t voff = (uint32_t)(srow - wgrp * kGroup) * (uint32_t)a.v_st + scol;
+  // (from the chunk's first row where ONE: its 64 rows lie within 2^31 bytes)
+  uint32_t kpiece[ONE ? NP : 1], vpiece[ONE ? NP : 1];
+#pragma unroll
+  for (int i = 0; i < (ONE ? NP : 1); ++i) {
+    const uint32_t from = (uint32_t)(ONE ? srow + i * RPP : srow - wgrp * kGroup);
+    kpiece[i] = from * (uint32_t)a.k_st + scol;
+    vpiece[i] = from * (uint32_t)a.v_st + scol;
+  }
   // ONE: read through the scalar cache (constant address space)
   using Table = std::conditional_t<ONE, const __attribute__((address_space(4))) int32_t*, const int32_t*>;
   const Table bt = (Table)(a.block_table + (int64_t)r * a.bt_sr);
@@ -199,11 +204,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     float gk, gv;
     int page;
   };
-  Fetched fa, fb;                    // of the odd and the even chunks to come
+  Fetched f;
   auto page_of = [&](int u) __attribute__((always_inline)) {
     return bt[block_of(min(base_of(min(u, u_hi - 1)) + lq * kGroup, t.end - 1))];
   };
-  auto fetch = [&](int u, Fetched& f) __attribute__((always_inline)) {
+  auto fetch = [&](int u) __attribute__((always_inline)) {
     const int j = base_of(min(u, u_hi - 1));
     f.page = pgn;
     const int page = pgn >= 0 && pgn < a.num_pages ? pgn : 0;
@@ -214,17 +219,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     const uint64_t ko = offset(page, a.k_sp) + offset(rw, a.k_st), vo = offset(page, a.v_sp) + offset(rw, a.v_st);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int q = D == 128 ? i : wgrp + 2 * i;                    // the piece's group: RPP is 16 or 32 rows
       const uint8_t *kp, *vp;
       if constexpr (ONE) {
-        kp = kcache + (ko + offset(q * kGroup, a.k_st));
-        vp = vcache + (vo + offset(q * kGroup, a.v_st));
+        kp = kcache + ko + kpiece[i];
+        vp = vcache + vo + vpiece[i];
       } else {
-        kp = kcache + lane_u64(ko, q);
-        vp = vcache + lane_u64(vo, q);
+        const int q = D == 128 ? i : wgrp + 2 * i;                  // the piece's group: RPP is 16 or 32 rows
+        kp = kcache + lane_u64(ko, q) + kpiece[0];
+        vp = vcache + lane_u64(vo, q) + vpiece[0];
       }
-      f.kb[i] = *reinterpret_cast<const uint2*>(kp + koff);
-      f.vb[i] = *reinterpret_cast<const uint2*>(vp + voff);
+      f.kb[i] = *reinterpret_cast<const uint2*>(kp);
+      f.vb[i] = *reinterpret_cast<const uint2*>(vp);
     }
   };
   // rows at positions lo .. hi each see every key of the chunk at j
@@ -232,7 +237,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     return j + kChunk - 1 <= lo && j + kChunk <= t.kend && (a.window == 0 || j > hi - a.window || j + kChunk <= a.sinks);
   };
   uint32_t nans = 0;                 // not 0: this thread met such a NaN
-  auto stage = [&](int u, int buf, Fetched& f) __attribute__((always_inline)) {
+  auto stage = [&](int u, int buf) __attribute__((always_inline)) {
     const int j = base_of(u);
     const bool ok = f.page >= 0 && f.page < a.num_pages && j + lq * kGroup < t.end;
     const uint32_t oks = ONE ? (ok ? 15u : 0u) : (uint32_t)__ballot(ok) & 15u;
@@ -285,104 +290,118 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   float m = -INFINITY, msub = 0.f, thr = -INFINITY, l = 0.f;
 
   if (u_lo < u_hi) {
-    // the pages of the first chunks at once: loads return in order
-    const int p0 = page_of(u_lo), p1 = page_of(u_lo + 1), p2 = page_of(u_lo + 2), p3 = page_of(u_lo + 3);
+    const int p0 = page_of(u_lo), p1 = page_of(u_lo + 1), p2 = page_of(u_lo + 2);
     pgn = p0;
-    fetch(u_lo, fb);
+    fetch(u_lo);
+    stage(u_lo, 0);
     pgn = p1;
-    fetch(u_lo + 1, fa);
-    stage(u_lo, 0, fb);
+    fetch(u_lo + 1);
     pgn = p2;
-    fetch(u_lo + 2, fb);
-    pgn = p3;
   }
   settle(qf);
   __syncthreads();
-  // one chunk: the next one (in f) goes to the other buffer, f takes the third next
-  // (converted last, beside the last products: first, the window case took 5% longer)
-  auto step = [&](int u, int buf, Fetched& f) __attribute__((always_inline)) {
+  // One chunk.  The next one (in f) goes to the other buffer first, and f takes the
+  // one after: the conversions fill the time of the products K Q^T, 6 of them per
+  // product (after the products P V instead: 2,048 rows after 30,720 keys 410 -> 405
+  // us, seven short prompts on 16-key pages 22.8 -> 21.6).  405 us are 822 TFLOP/s,
+  // and orders, depths and waits of the loads no longer move it: at the clocks that
+  // so many products leave, the matrix cores and the vector units are each busy for
+  // half of the time.
+  auto step = [&](int u, int buf) __attribute__((always_inline)) {
     const uint16_t* sK = reinterpret_cast<const uint16_t*>(smem + buf * L::buf);
     const uint16_t* sV = reinterpret_cast<const uint16_t*>(smem + buf * L::buf + L::kBytes);
     const float4* sg = reinterpret_cast<const float4*>(smem + buf * L::buf + L::kBytes + L::vBytes);
     const int j0 = base_of(u);
-    // wave-uniform: does some row see a key, does every row see every key
-    const bool some = wave_live && j0 <= wpmax && (a.window == 0 || j0 + kChunk - 1 > wpmin - a.window || j0 < a.sinks);
-    if (some) {
-      float4 gs[4];                                 // (ONE: four times the same)
+    stage(min(u + 1, u_hi - 1), buf ^ 1);
+    fetch(u + 2);
+    pgn = page_of(u + 3);
+    float4 gs[4];                                 // (ONE: four times the same)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) gs[q] = sg[ONE ? 0 : q];
-      // (a group without a page has K zero and an exponent of -inf, and needs no mask)
-      const bool whole = seen_whole(j0, wpmin, wpmax);
-      f32x16_t s[2];
+    for (int q = 0; q < 4; ++q) gs[q] = sg[ONE ? 0 : q];
+    // (a group without a page has K zero and an exponent of -inf, and needs no mask)
+    const bool whole = seen_whole(j0, wpmin, wpmax);
+    f32x16_t s[2];
+    // K's operands, kAhead of them in flight
+    constexpr int kAhead = 4;
+    uint4 kf[kAhead];
+    auto k_operand = [&](int i) {
+      return *reinterpret_cast<const uint4*>(sK + (32 * (i / KS) + rl) * KP + 16 * (i % KS) + 8 * hh);
+    };
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        s[kt] = zero16();
+    for (int f = 0; f < kAhead; ++f) kf[f] = k_operand(f);
+    s[0] = s[1] = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          s[kt] = Mfma<T>::mac(*reinterpret_cast<const uint4*>(sK + (32 * kt + rl) * KP + 16 * ks + 8 * hh), qf[ks], s[kt]);
-      }
+    for (int f = 0; f < 2 * KS; ++f) {
+      s[f / KS] = Mfma<T>::mac(kf[f % kAhead], qf[f % KS], s[f / KS]);
+      if (f + kAhead < 2 * KS) kf[f % kAhead] = k_operand(f + kAhead);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead + (ONE ? 1 : 4), 0);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float b = gs[q].y - msub;
+    for (int f = 0; f < 2 * KS; ++f) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (f < 2 * KS - kAhead) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[q / 2][8 * (q % 2) + j] = fmaf(s[q / 2][8 * (q % 2) + j], gs[q].x, b);
-      }
-      if (per_lane(!whole)) {
+    for (int q = 0; q < 4; ++q) {
+      const float b = gs[q].y - msub;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const int k = j0 + 4 * hh + 32 * kt + 8 * (x / 4) + x % 4;
-            const bool see = ((uint32_t)(k - my_lo) < my_span) | ((uint32_t)k < my_first);
-            s[kt][x] = see ? s[kt][x] : -INFINITY;
-          }
-      }
-      float zm = s[0][0];
-#pragma unroll
-      for (int x = 1; x < 16; ++x) zm = fmaxf(zm, s[0][x]);
-#pragma unroll
-      for (int x = 0; x < 16; ++x) zm = fmaxf(zm, s[1][x]);
-      if (per_lane(__any(zm > thr))) {
-        const float mn = fmaxf(m, xor32_max(zm) + msub - kBelow);
-        const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
-        const float now = mn == -INFINITY ? 0.f : mn, by = msub - now;
-        m = mn;
-        msub = now;
-        thr = mn == -INFINITY ? -INFINITY : kBelow + kSlack;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < MT; ++d)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[d][x] *= alpha;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) s[kt][x] += by;
-      }
+      for (int j = 0; j < 8; ++j) s[q / 2][8 * (q % 2) + j] = fmaf(s[q / 2][8 * (q % 2) + j], gs[q].x, b);
+    }
+    if (per_lane(!whole)) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float pe[8], sum;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) pe[j] = __builtin_amdgcn_exp2f(s[kt][8 * q + j]);
-          const uint4 pf = make_uint4(pack_f16(pe[0], pe[1]), pack_f16(pe[2], pe[3]), pack_f16(pe[4], pe[5]),
-                                      pack_f16(pe[6], pe[7]));
-          sum = ((pe[0] + pe[1]) + (pe[2] + pe[3])) + ((pe[4] + pe[5]) + (pe[6] + pe[7]));
-          l = fmaf(sum, gs[2 * kt + q].z, l);
-#pragma unroll
-          for (int d = 0; d < MT; ++d)
-            o[d] = Mfma<__half>::mac(a_operand_tr<VP>(sV, 32 * kt + 16 * q, 32 * d, lane), pf, o[d]);
+        for (int x = 0; x < 16; ++x) {
+          const int k = j0 + 4 * hh + 32 * kt + 8 * (x / 4) + x % 4;
+          const bool see = ((uint32_t)(k - my_lo) < my_span) | ((uint32_t)k < my_first);
+          s[kt][x] = see ? s[kt][x] : -INFINITY;
         }
     }
-    stage(min(u + 1, u_hi - 1), buf ^ 1, f);
-    fetch(u + 3, f);
-    pgn = page_of(u + 4);
+    float zm = s[0][0];
+#pragma unroll
+    for (int x = 1; x < 16; ++x) zm = fmaxf(zm, s[0][x]);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) zm = fmaxf(zm, s[1][x]);
+    uint4 vf[MT];
+#pragma unroll
+    for (int d = 0; d < MT; ++d) vf[d] = a_operand_tr<VP>(sV, 0, 32 * d, lane);
+    if (per_lane(__any(zm > thr))) {
+      const float mn = fmaxf(m, xor32_max(zm) + msub - kBelow);
+      const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
+      const float now = mn == -INFINITY ? 0.f : mn, by = msub - now;
+      m = mn;
+      msub = now;
+      thr = mn == -INFINITY ? -INFINITY : kBelow + kSlack;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < MT; ++d)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[d][x] *= alpha;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[kt][x] += by;
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float pe[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pe[j] = __builtin_amdgcn_exp2f(s[g / 2][8 * (g % 2) + j]);
+      const uint4 pf = make_uint4(pack_f16(pe[0], pe[1]), pack_f16(pe[2], pe[3]), pack_f16(pe[4], pe[5]),
+                                  pack_f16(pe[6], pe[7]));
+      l = fmaf(((pe[0] + pe[1]) + (pe[2] + pe[3])) + ((pe[4] + pe[5]) + (pe[6] + pe[7])), gs[g].z, l);
+#pragma unroll
+      for (int d = 0; d < MT; ++d) {
+        o[d] = Mfma<__half>::mac(vf[d], pf, o[d]);
+        if (g < 3) vf[d] = a_operand_tr<VP>(sV, 16 * g + 16, 32 * d, lane);
+      }
+    }
     __syncthreads();
   };
   for (int u = u_lo; u < u_hi; u += 2) {
-    step(u, 0, fa);
-    if (u + 1 < u_hi) step(u + 1, 1, fb);
+    step(u, 0);
+    if (u + 1 < u_hi) step(u + 1, 1);
   }
 
   if constexpr (KV == kFp8E4M3FN) {
@@ -556,8 +575,9 @@ int launch_tiles(const PrefillK& p, unsigned grid, hipStream_t st) {
 }
 template <typename T, int KV, int D>
 int launch(const PrefillK& p, unsigned grid, hipStream_t st) {
-  const int rc = p.a.page_size % kChunk == 0 ? launch_tiles<T, KV, D, true>(p, grid, st)
-                                             : launch_tiles<T, KV, D, false>(p, grid, st);
+  const bool one = p.a.page_size % kChunk == 0 && std::max(p.a.k_st, p.a.v_st) <= INT32_MAX / kChunk;
+  const int rc = one ? launch_tiles<T, KV, D, true>(p, grid, st)
+                     : launch_tiles<T, KV, D, false>(p, grid, st);
   if (rc != SRSWA_OK) return rc;
   if (p.nsplit > 1)
     cache8_join_kernel<T, D><<<(unsigned)(p.a.HKV * p.tiles * 4), 2 * D, 0, st>>>(p);
