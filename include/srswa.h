@@ -1024,10 +1024,11 @@ int srswa_cache8_append(const srswa_cache8_append_args* a, void* stream);
  *   topk:      (decode only) the window keys j > p - window without a bias, and
  *              the keys before the window of the listed blocks (page_size keys
  *              each, -1 = empty, a repeated id counts once) with the slot's bias.
- * A row without a visible key gives 0 (lse -inf).  Rows of q beyond the
- * requests' are left as they are.  P and V are multiplied in fp16 (V's bytes are
+ * A row without a visible key gives 0 (lse -inf).  A NaN in V reaches the rows
+ * that see its key.  Rows of q beyond the requests' are left as they are.  P and V are multiplied in fp16 (V's bytes are
  * exact there), q and K in q's type; sums and statistics are fp32.  Scales are
- * positive; a V scale below 2^-100 counts as 2^-100.
+ * positive; a V scale below 2^-100 counts as 2^-100.  Cache strides are below
+ * 2^31 bytes, token strides below 2^28.
  * srswa_cache8_decode: a few rows per request (max_query_len each when
  * cu_seqlens_q is NULL), split over the keys; srswa_cache8_prefill: many. */
 typedef struct {
