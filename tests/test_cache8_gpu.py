@@ -413,6 +413,28 @@ def test_ctypes_path_gives_the_same(dev, monkeypatch):
         assert torch.equal(a, b)
 
 
+def test_arguments_of_other_kinds(dev):
+    """Numbers that are not Python's own, truth values that are not bools, an output of a wider tensor."""
+    import numpy as np
+    from srswa import cache8
+    g = torch.Generator().manual_seed(62)
+    c = dict(page=16, HQ=4, HKV=2, D=64, W=4, kv=torch.int8)
+    table, kc, vc, ks, vs = _state(c, g, [50, 20])
+    q = torch.randn(4, 4, 64, generator=g).to(BF).to(dev)
+    args = [t.to(dev) for t in (kc, vc, ks, vs)] + [torch.tensor(table, dtype=torch.int32).to(dev)]
+    sl, cu = torch.tensor([50, 20], dtype=torch.int32).to(dev), torch.tensor([0, 2, 4], dtype=torch.int32).to(dev)
+    want = cache8.cache8_decode(q, *args, sl, scale=0.5, decode_query_len=2, window=9, sinks=2, return_lse=True)
+    wide = torch.empty(4, 9, 64, dtype=BF, device=dev)
+    for kw in (dict(return_lse=1), dict(return_lse=np.True_), dict(return_lse=True, out=wide[:, 3:7])):
+        runs = [cache8.cache8_decode(q, *args, sl, scale=np.float32(0.5), decode_query_len=np.int64(2),
+                                     window=np.int32(9), sinks=np.int64(2), **kw),
+                cache8.cache8_decode(q, *args, sl, scale=0.5, decode_query_len=2, window=9, sinks=2, **kw),
+                cache8.cache8_prefill(q, *args, cu, sl, 2, scale=0.5, window=9, sinks=2, **kw)]
+        for got in runs:
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.is_tensor(cache8.cache8_decode(q, *args, sl, scale=0.5, decode_query_len=2, return_lse=0))
+
+
 def test_empty_calls(dev):
     from srswa import cache8
     kc = torch.zeros(3, 16, 1, 64, dtype=torch.int8, device=dev)

@@ -191,7 +191,7 @@ def cache8_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, 
     w, s = _window(window, sinks)
     if _lib.host:
         got = _lib.host.attend(0, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, None, decode_query_len,
-                               scale, w, s, out, return_lse, None, None)
+                               scale, w, s, out, bool(return_lse), None, None)
         if got is not NotImplemented:
             return got
     dql = int(decode_query_len)
@@ -218,7 +218,7 @@ def cache8_prefill(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlen
     w, s = _window(window, sinks)
     if _lib.host:
         got = _lib.host.attend(1, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens_q,
-                               max_query_len, scale, w, s, out, return_lse, None, None)
+                               max_query_len, scale, w, s, out, bool(return_lse), None, None)
         if got is not NotImplemented:
             return got
     if q.dim() != 3 or int(max_query_len) < 0:
