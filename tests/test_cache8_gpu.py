@@ -486,6 +486,32 @@ def test_prefill_tiles_match_oracle(dev, name, kv):
     _check(got, lse, ref, name)
 
 
+@pytest.mark.parametrize("bound", [1, 3, 50, 600])
+def test_rows_past_the_bound_are_left(dev, bound):
+    """Requests longer than max_query_len: their first rows are right, the others untouched."""
+    from srswa import cache8
+    g = torch.Generator().manual_seed(172)
+    c = dict(page=64, HQ=8, HKV=2, D=64, W=60, kv=torch.int8)
+    n, ctx = [70, 2, 650, 5], [3000, 10, 100, 2500]
+    lens = [a + b for a, b in zip(n, ctx)]
+    table, kc, vc, ks, vs = _state(c, g, lens)
+    cu = [0, 70, 72, 722, 727]
+    q = torch.randn(727, 8, 64, generator=g).to(BF)
+    keep = [i for r in range(4) for i in range(cu[r], cu[r] + min(n[r], bound))]
+    some = sorted(set(keep[:40] + keep[-40:]))            # (the oracle is slow)
+    cuts = [sum(1 for i in some if i < x) for x in cu]
+    out = torch.full(q.shape, 7.0, dtype=BF, device=dev)
+    cache8.cache8_prefill(*(t.to(dev) for t in (q, kc, vc, ks, vs)), torch.tensor(table, dtype=torch.int32).to(dev),
+                          torch.tensor(cu).to(dev), torch.tensor(lens).to(dev), bound, scale=0.125, out=out)
+    rest = [i for i in range(727) if i not in set(keep)]
+    assert (out[rest] == 7.0).all()
+    for r in range(4):
+        rows = some[cuts[r]:cuts[r + 1]]
+        for i in rows:                                    # one row at a time: its own length
+            o, _, tol = O.attend(q[i:i + 1], kc, vc, ks, vs, [table[r]], [0, 1], [lens[r] - (cu[r + 1] - 1 - i)], 0.125)
+            assert ((out[i:i + 1].cpu().double() - o).abs() <= tol).all(), (bound, i)
+
+
 @pytest.mark.parametrize("bound", [0, WIDE])
 def test_prefill_of_many_requests(dev, bound):
     """More requests than a wave has lanes: each workgroup finds its own."""

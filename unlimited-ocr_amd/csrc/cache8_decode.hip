@@ -72,6 +72,7 @@ __device__ __forceinline__ Tile tile_of(const AttendK& p, int r, int tile) {
   t.r = r;
   const int q0 = a.cu_seqlens_q ? min(max(a.cu_seqlens_q[r], 0), a.total_q) : r * a.max_query_len;
   const int q1 = a.cu_seqlens_q ? min(max(a.cu_seqlens_q[r + 1], q0), a.total_q) : q0 + a.max_query_len;
+  const int ql = min(q1 - q0, a.max_query_len);          // (later rows are not written; records hold no more)
   const int sl = max(a.seq_lens[r], 0);
   t.q0 = q0;
   t.p0 = sl - (q1 - q0);
@@ -79,10 +80,10 @@ __device__ __forceinline__ Tile tile_of(const AttendK& p, int r, int tile) {
     const int per = (p.G + kRows - 1) / kRows;
     const int tok = tile / per, g0 = tile % per * kRows;
     t.row0 = tok * p.G + g0;
-    t.nrows = tok < q1 - q0 ? min(kRows, p.G - g0) : 0;
+    t.nrows = tok < ql ? min(kRows, p.G - g0) : 0;
   } else {
     t.row0 = tile * kRows;
-    t.nrows = (int)max((int64_t)0, min((int64_t)kRows, (int64_t)(q1 - q0) * p.G - t.row0));
+    t.nrows = (int)max((int64_t)0, min((int64_t)kRows, (int64_t)ql * p.G - t.row0));
   }
   t.kend = (int)min((int64_t)sl, (int64_t)a.max_blocks * a.page_size);
   t.pmin = t.p0 + t.row0 / p.G;
