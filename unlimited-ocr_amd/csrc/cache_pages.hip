@@ -301,11 +301,14 @@ __global__ __launch_bounds__(kThreads) void reorder_deal_kernel(PagesK p) {
   reorder_deal(p, s, s_row, s_hit, &s_nhit);
 }
 
-// The four steps in one workgroup, for up to kWide rows and 32 kWide pages, the
-// marks and the list of free pages in LDS: a power of two of threads per row, every
-// row at once where they suffice (64 rows of 128 pages 13 us; the same steps through
-// memory 24 us).
+// The four steps in one workgroup, the marks and the list of free pages in LDS: a power
+// of two of threads per row, every row at once where they suffice.  Against the four
+// launches, one layer's copies included: 4 rows of 128 pages 9.5 us (17.6), 64 rows 16.5
+// (23.1), 128 rows 29.6 (29.3), 256 rows 54 (32); 8 rows of a pool of 32,000 pages 23.5
+// (18.6).
 constexpr int kWide = 1024;
+constexpr int kPlanRows = 128, kPlanEntries = 16384, kPlanPages = 16384;
+static_assert(kPlanRows <= kWide && kPlanPages <= 32 * kWide, "a thread per row, a bit per page");
 __global__ __launch_bounds__(kWide) void reorder_plan_kernel(PagesK p) {
   __shared__ int s[kWide / kWave];
   __shared__ int s_par[kWide], s_len[kWide], s_src[kWide], s_free[kWide];
@@ -623,7 +626,7 @@ extern "C" int srswa_pages_reorder(const srswa_pages_args* a, void* ws, size_t w
   const int rc = setup(a, ws, ws_bytes, true, "pages reorder", &k);
   if (rc != SRSWA_OK) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (k.R <= kWide && (int64_t)k.R * k.W <= 32768 && k.N <= 32 * kWide) {
+  if (k.R <= kPlanRows && (int64_t)k.R * k.W <= kPlanEntries && k.N <= kPlanPages) {
     reorder_plan_kernel<<<1, kWide, 0, st>>>(k);
   } else {
     copy_ref_kernel<<<(unsigned)((k.N + kThreads - 1) / kThreads), kThreads, 0, st>>>(k);
