@@ -39,7 +39,10 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kRows = 16;
 constexpr float kBelow = 7.f, kSlack = 8.f;   // the running maximum's place and play (log2)
 constexpr int kGroup = 16;     // keys per page lookup; a unit is two groups
-constexpr int kMinShare = 16;  // units of the smallest share
+constexpr int kMergeWaves = 8;
+// units of the smallest share: one request of 9,000 keys 19.2 us with 8, 17.9 with 16,
+// 19.9 with 32; of 3,000 keys 14.5, 15.5, 20.4
+constexpr int kMinShare = 16;
 
 struct AttendK {
   srswa_cache8_attend_args a;
@@ -313,7 +316,8 @@ __device__ __forceinline__ void attend_item(const AttendK& p, int h, const Tile&
 
     // One unit's bytes are held at a time: K's registers are loaded again as soon as
     // the products have read them, V's after the transposes, so a unit's K comes in
-    // behind the softmax and its V behind the next products, and four waves fit a SIMD
+    // behind the softmax and its V behind the next products, and three waves fit a SIMD
+    // (in the registers of four the loop spills: 48 uneven requests 297 us, not 220)
     UnitBytes<D> b;
     auto load_k = [&](int i) __attribute__((always_inline)) {
       i = min(i, cnt - 1);                       // (past the end: the last unit again, not used)
@@ -565,14 +569,16 @@ __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
   }
 }
 
-// Joins the shares of an item that was cut: one wave per (item, kv head, row), D / 64
-// dims a lane.  Share i begins with the item (its first record) unless the item
-// starts inside it (its last).
+// Joins the shares of an item that was cut: one workgroup per (item, kv head, row), a
+// wave for each eighth record, D / 64 dims a lane.  Share i begins with the item (its
+// first record) unless the item starts inside it (its last).  One request of 30,000
+// keys, 59 records a row: 42.9 us with one wave, 29.8 with four, 28.8 with eight.
 template <typename T, int D, bool SEL>
-__global__ __launch_bounds__(kWave) void cache8_merge_kernel(AttendK p) {
+__global__ __launch_bounds__(kMergeWaves * kWave) void cache8_merge_kernel(AttendK p) {
   constexpr int DL = D / kWave;
+  __shared__ float s_o[kMergeWaves][D], s_l[kMergeWaves];
   const srswa_cache8_attend_args& a = p.a;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int rr = (int)blockIdx.x % p.rs, h = (int)blockIdx.x / p.rs % a.HKV, item = (int)blockIdx.x / p.rs / a.HKV;
   const Tile t = tile_of<SEL>(p, item / p.tiles, item % p.tiles);
   if (rr >= t.nrows) return;
@@ -601,22 +607,25 @@ __global__ __launch_bounds__(kWave) void cache8_merge_kernel(AttendK p) {
   for (int i = s0 + lane; i <= s1; i += kWave) M = fmaxf(M, record(i)[p.rs * D + rr]);
   M = wave_max(M);
   float o[DL] = {}, L = 0.f;
-  for (int i0 = s0; i0 <= s1; i0 += kWave) {
-    const int cnt = min(kWave, s1 - i0 + 1);
-    float f = 0.f, lk = 0.f;                     // lane k: share i0 + k
-    if (lane < cnt) {
-      const float* rec = record(i0 + lane);
-      const float mk = rec[p.rs * D + rr];
-      f = mk == -INFINITY ? 0.f : exp2f(mk - M);
-      lk = f * rec[p.rs * D + p.rs + rr];
-    }
-    L += wave_sum(lk);
-    for (int k = 0; k < cnt; ++k) {
-      const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k));
-      const float* rec = record(i0 + k) + rr * D + DL * lane;
+#pragma unroll 8
+  for (int i = s0 + wave; i <= s1; i += kMergeWaves) {
+    const float* rec = record(i);
+    const float mk = rec[p.rs * D + rr];
+    const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
+    L = fmaf(f, rec[p.rs * D + p.rs + rr], L);
 #pragma unroll
-      for (int d = 0; d < DL; ++d) o[d] = fmaf(fk, rec[d], o[d]);
-    }
+    for (int d = 0; d < DL; ++d) o[d] = fmaf(f, rec[rr * D + DL * lane + d], o[d]);
+  }
+#pragma unroll
+  for (int d = 0; d < DL; ++d) s_o[wave][DL * lane + d] = o[d];
+  if (lane == 0) s_l[wave] = L;
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 1; w < kMergeWaves; ++w) {
+    L += s_l[w];
+#pragma unroll
+    for (int d = 0; d < DL; ++d) o[d] += s_o[w][DL * lane + d];
   }
   const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
   const float inv = inv_sum(M, L);
@@ -697,8 +706,9 @@ namespace {
 // Short items are taken whole, others shared by as many workgroups as the GPU holds
 // at once.  Whole needs no second launch and no count of the items, but leaves CUs
 // idle where the workgroups are few: one request of ten heads 9.6 us whole against
-// 15.2 shared at 777 keys, 21.5 against 16.8 at 3,000 (94 units); 24 requests of
-// 400 to 3,000 keys 23 against 31.
+// 14.9 shared at 777 keys, 21.6 against 15.4 at 3,000 (94 units); four of 1,000 to
+// 4,000 keys 24.1 against 20.4, eight 25.4 against 25.0, 24 of 400 to 3,000 keys 23.1
+// against 30.9, 24 of 400 to 6,000 keys 48.2 against 43.5.
 AttendK plan(const srswa_cache8_attend_args* a) {
   AttendK p{};
   p.a = *a;
@@ -719,7 +729,7 @@ AttendK plan(const srswa_cache8_attend_args* a) {
   p.pairs = a->D == 64 && a->HKV % 2 == 0;
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
-  if (units > 128 || (units > 64 && wgs < 40))
+  if (units > 128 || (units > 64 && wgs <= 64))
     p.shares = (int)std::min<int64_t>(std::max(1, (a->D == 64 ? 4 : 3) * cus / a->HKV), (units * p.items + kMinShare - 1) / kMinShare);
   return p;
 }
@@ -736,7 +746,7 @@ void launch(const AttendK& p, unsigned grid, hipStream_t st) {
   if (kMix && p.a.max_query_len > 1) cache8_decode_kernel<T, KV, D, SEL, kMix, 4><<<grid, 4 * kWave, 0, st>>>(p);
   else cache8_decode_kernel<T, KV, D, SEL, false, 4><<<grid, 4 * kWave, 0, st>>>(p);
   if (p.shares > 0)
-    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.items * p.a.HKV * p.rs), kWave, 0, st>>>(p);
+    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.items * p.a.HKV * p.rs), kMergeWaves * kWave, 0, st>>>(p);
 }
 template <typename T, int KV, int D>
 void launch_sel(const AttendK& p, unsigned grid, hipStream_t st) {
