@@ -455,9 +455,16 @@ def test_empty_calls(dev):
     assert not kc.any() and (s == 1).all()
 
 
-# A bound above the longest request: the work it allows for takes 128-row tiles, which
-# short prompts of a tight bound do not.
+# Small cases take the form by items of 16 rows; these run them through the 128-row tiles
+# too, with a bound on the longest request that is far above it.
 WIDE = 1 << 15
+
+
+@pytest.fixture
+def form(monkeypatch):
+    def take(bound):
+        monkeypatch.setenv("SRSWA_CACHE8_PREFILL", "tiles" if bound == WIDE else "items")
+    return take
 
 
 def _prefill(dev, c, g, bound, spoil=None, q=None):
@@ -480,16 +487,19 @@ def _prefill(dev, c, g, bound, spoil=None, q=None):
 
 @pytest.mark.parametrize("kv", [torch.int8, E4M3])
 @pytest.mark.parametrize("name", list(PREFILL))
-def test_prefill_tiles_match_oracle(dev, name, kv):
+def test_prefill_tiles_match_oracle(dev, form, name, kv):
+    form(WIDE)
     g = torch.Generator().manual_seed(list(PREFILL).index(name) + 160)
     got, lse, ref = _prefill(dev, dict(PREFILL[name], kv=kv), g, WIDE)
     _check(got, lse, ref, name)
 
 
+@pytest.mark.parametrize("tiles", [False, True])
 @pytest.mark.parametrize("bound", [1, 3, 50, 600])
-def test_rows_past_the_bound_are_left(dev, bound):
+def test_rows_past_the_bound_are_left(dev, form, bound, tiles):
     """Requests longer than max_query_len: their first rows are right, the others untouched."""
     from srswa import cache8
+    form(WIDE if tiles else 0)
     g = torch.Generator().manual_seed(172)
     c = dict(page=64, HQ=8, HKV=2, D=64, W=60, kv=torch.int8)
     n, ctx = [70, 2, 650, 5], [3000, 10, 100, 2500]
@@ -513,14 +523,44 @@ def test_rows_past_the_bound_are_left(dev, bound):
 
 
 @pytest.mark.parametrize("bound", [0, WIDE])
-def test_prefill_of_many_requests(dev, bound):
+def test_prefill_of_many_requests(dev, form, bound):
     """More requests than a wave has lanes: each workgroup finds its own."""
+    form(bound)
     g = torch.Generator().manual_seed(171)
     n = torch.randint(0, 9, (150,), generator=g).tolist()
     n[70], n[149] = 140, 33
     c = dict(page=16, HQ=4, HKV=2, D=64, kv=E4M3, q=n, ctx=torch.randint(0, 20, (150,), generator=g).tolist(), W=10)
     got, lse, ref = _prefill(dev, c, g, bound)
     _check(got, lse, ref, "150 requests")
+
+
+def test_prefill_takes_either_form_by_itself(dev):
+    """Shapes on both sides of the choice, the same requests cut into calls of few rows
+    and in one of many: equal within the forms' roundings."""
+    from srswa import cache8
+    g = torch.Generator().manual_seed(173)
+    page, HQ, HKV, D, R = 64, 16, 8, 64, 4
+    n, ctx = 700, 300
+    table, pages = _table(g, [n + ctx] * R, page, 16)
+    kc, ks = _cache(g, pages, page, HKV, D, E4M3)
+    vc, vs = _cache(g, pages, page, HKV, D, E4M3)
+    q = torch.randn(R, n, HQ, D, generator=g).to(HF).to(dev)
+    args = [t.to(dev) for t in (kc, vc, ks, vs)] + [torch.tensor(table, dtype=torch.int32).to(dev)]
+
+    def run(lo, hi):
+        cu = torch.arange(R + 1, dtype=torch.int32, device=dev) * (hi - lo)
+        sl = torch.full((R,), ctx + hi, dtype=torch.int32, device=dev)
+        o, lse = cache8.cache8_prefill(q[:, lo:hi].reshape(-1, HQ, D), *args, cu, sl, hi - lo, scale=0.125,
+                                       return_lse=True)
+        return o.reshape(R, hi - lo, HQ, D).double(), lse.reshape(R, hi - lo, HQ).double()
+
+    whole = run(0, n)
+    parts = [run(lo, min(lo + 9, n)) for lo in range(0, n, 9)]
+    o, lse = (torch.cat([p[i] for p in parts], 1) for i in range(2))
+    # each form: weights within 2^-11 of a half step in fp16 and an output rounding of 2^-11, of values up to max |v|
+    top = (vc.float().abs().amax((1, 3)) * vs).amax().item()
+    assert ((whole[0] - o).abs() <= 4 * 2.0 ** -11 * top).all()
+    assert ((whole[1] - lse).abs() <= 1e-4 * (1 + lse.abs())).all()
 
 
 def _check_nan(got, lse, ref, what):
@@ -551,9 +591,10 @@ NANS = {
 @pytest.mark.parametrize("what", ["k", "v", "q"])
 @pytest.mark.parametrize("bound", [0, WIDE])
 @pytest.mark.parametrize("name", list(NANS))
-def test_prefill_keeps_a_nan_to_the_rows_that_see_it(dev, name, bound, what):
+def test_prefill_keeps_a_nan_to_the_rows_that_see_it(dev, form, name, bound, what):
     """A stored NaN reaches the rows that see its key, in V its own dim only; a
     query's NaN its own row."""
+    form(bound)
     c = dict(NANS[name], kv=E4M3)
     g = torch.Generator().manual_seed(181)
 
@@ -589,8 +630,9 @@ def test_decode_keeps_a_nan_to_the_rows_that_see_it(dev, D):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-def test_the_smallest_and_largest_v_scales(dev, dtype):
+def test_the_smallest_and_largest_v_scales(dev, form, dtype):
     """A cache of zeros (scale 2^-100) and, in bf16, the largest finite values."""
+    form(WIDE)
     from srswa import cache8
     g = torch.Generator().manual_seed(201)
     table, n = _table(g, [600, 600], 16, 38)
@@ -635,7 +677,7 @@ def test_decode_and_append_of_many_requests(dev):
            "130 requests")
 
 
-def test_offsets_past_32_bits(dev):
+def test_offsets_past_32_bits(dev, form):
     """Pages more than 2^32 bytes into a cache: append, decode, prefill and a page copy there."""
     from srswa import cache8, cache_pages
     g = torch.Generator().manual_seed(231)
@@ -659,6 +701,7 @@ def test_offsets_past_32_bits(dev):
     q = torch.randn(2 * 40, H, D, generator=g).to(BF)
     ref = O.attend(q, kc, vc, ks, vs, table, [0, 40, 80], lens, 0.1)
     for bound in (40, WIDE):
+        form(bound)
         got = cache8.cache8_prefill(q.to(dev), *state, far_table, torch.tensor([0, 40, 80]).to(dev), sl, bound, scale=0.1,
                                     return_lse=True)
         _check(*got, ref, bound)
@@ -674,7 +717,7 @@ def test_offsets_past_32_bits(dev):
     _check(o, lse, one, "forked")
 
 
-def test_a_page_s_rows_far_apart(dev):
+def test_a_page_s_rows_far_apart(dev, form):
     """A cache stored by place in the page first: token strides past 2^25 bytes."""
     from srswa import cache8
     g = torch.Generator().manual_seed(241)
@@ -692,6 +735,7 @@ def test_a_page_s_rows_far_apart(dev):
     q = torch.randn(80, H, D, generator=g).to(BF)
     ref = O.attend(q, kc, kc, ks, vs, table, [0, 40, 80], lens, 0.1)
     for bound in (40, WIDE):
+        form(bound)
         got = cache8.cache8_prefill(q.to(dev), far, far, sk, sv, bt, torch.tensor([0, 40, 80]).to(dev),
                                     torch.tensor(lens).to(dev), bound, scale=0.1, return_lse=True)
         _check(*got, ref, bound)

@@ -134,8 +134,9 @@ __device__ __forceinline__ uint2 bytes4_to(uint32_t w) {
 int cache8_check(const srswa_cache8_attend_args* a, const char* what);
 int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream, const char* what);
 size_t cache8_decode_ws(const srswa_cache8_attend_args* a);
-// the (item, kv head) pairs of that form, and the units of 32 keys of one at most
-void cache8_decode_load(const srswa_cache8_attend_args* a, int64_t* wgs, int64_t* units);
+// what that form does for a call: (item, kv head) pairs, units of 32 keys of one at most,
+// and whether they are shared out
+void cache8_decode_load(const srswa_cache8_attend_args* a, int64_t* wgs, int64_t* units, bool* shared);
 inline bool cache8_plannable(const srswa_cache8_attend_args* a) {
   return a && a->R > 0 && a->HQ > 0 && a->HKV > 0 && a->page_size >= 16 && a->max_blocks > 0 && a->max_query_len > 0;
 }

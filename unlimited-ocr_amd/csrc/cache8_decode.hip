@@ -788,10 +788,11 @@ int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_byt
 
 size_t cache8_decode_ws(const srswa_cache8_attend_args* a) { return ws_bytes_of(plan(a)); }
 
-void cache8_decode_load(const srswa_cache8_attend_args* a, int64_t* wgs, int64_t* units) {
+void cache8_decode_load(const srswa_cache8_attend_args* a, int64_t* wgs, int64_t* units, bool* shared) {
   const AttendK p = plan(a);
-  *wgs = (int64_t)a->R * p.tiles * a->HKV;
+  *wgs = std::min<int64_t>((int64_t)a->R * p.tiles, (int64_t)a->total_q * p.G / kRows + a->R) * a->HKV;
   *units = p.most_units;
+  *shared = p.shares > 0;
 }
 
 }  // namespace srswa

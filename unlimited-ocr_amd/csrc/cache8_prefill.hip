@@ -16,6 +16,8 @@
 // A chunk that every row of a wave sees whole takes no mask.  Parts (few tiles, long keys) write fp32 records that
 // cache8_join_kernel combines.
 #include <algorithm>
+#include <cstdlib>
+#include <cstring>
 
 #include "cache8.h"
 #include "mfma_common.h"
@@ -35,6 +37,7 @@ struct PrefillK {
   int G, tiles, nsplit;           // tiles: of all requests at most
   uint32_t page_mul;              // key / page_size = umulhi(key, page_mul) >> page_shift
   int page_shift;
+  int64_t chunks;                 // of a tile at most
   float scale_l2;
   bool by_group;                  // the tiles of a group to one XCD, else in turn
   float* part;                    // [tiles][HKV][nsplit][128 * (D + 2)]
@@ -532,6 +535,7 @@ PrefillK plan(const srswa_cache8_attend_args* a) {
   p.page_mul = (uint32_t)(((1ull << (31 + lg)) / a->page_size) + 1);
   int64_t keys = (int64_t)a->max_blocks * a->page_size;
   if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + kRowsWg / p.G + 2 * kChunk + a->sinks);
+  p.chunks = (keys + kChunk - 1) / kChunk;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, keys / kChunk / kMinChunks));
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
@@ -559,19 +563,35 @@ size_t ws_bytes_of(const PrefillK& p) {
   return p.nsplit > 1 ? (size_t)p.tiles * p.a.HKV * p.nsplit * kRowsWg * (p.a.D + 2) * sizeof(float) : 0;
 }
 
-// Few rows per request, or little work in all, take decode's form of 16-row items: a
-// 128-row tile converts each key once for eight times the rows, but fills fewer CUs
-// and takes longer to start and to end.  One request of ten heads, 16-row items
-// against tiles: 49 against 68 us (32 rows after 30,720 keys), 104 against 75 (128
-// rows), 11.5 against 22 (512 rows, no prefix); eight requests: 24.6 against 35 (64
-// rows after up to 2,000 keys), 41 against 31 (512 rows, no prefix).
-bool narrow(const srswa_cache8_attend_args* a) {
-  if ((int64_t)a->max_query_len * (a->HQ / a->HKV) <= 32) return true;
+// Whether decode's form of 16-row items is the faster: a 128-row tile converts each key
+// once for eight times the rows, but fills fewer CUs and takes longer to start and end.
+// Both are estimated in us from what 24 shapes measured (their keys are the table's
+// width here, a call's may be fewer, so near ties go to the items): items 14 shared out
+// or 8 whole, and 0.85 per unit of a place (three a CU) or 0.19 of the longest; tiles 10,
+// 20 with a join, and per chunk of a part 1.35 alone on a CU, 2.4 beside another.  One
+// request of ten heads, items against tiles: 33 against 62 us (16 rows after 30,000
+// keys), 64 against 64 (64 rows), 105 against 65 (128 rows), 47 against 34 (128 rows
+// after 8,000), 22 against 28 (256 after 2,000), 11 against 21 (512, no prefix); eight:
+// 25 against 29 (64 after 2,000), 22 against 16 (256, no prefix); sixteen of 16 rows
+// after 30,000 keys 152 against 264.
+// SRSWA_CACHE8_PREFILL = items or tiles takes that form for any call.
+bool narrow(const srswa_cache8_attend_args* a, const PrefillK& p) {
+  if (const char* form = std::getenv("SRSWA_CACHE8_PREFILL")) {
+    if (std::strcmp(form, "items") == 0) return true;
+    if (std::strcmp(form, "tiles") == 0) return false;
+  }
   int64_t wgs, units;
-  cache8_decode_load(a, &wgs, &units);
+  bool shared;
+  cache8_decode_load(a, &wgs, &units, &shared);
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
-  return wgs <= 3 * cus && wgs * units <= 156 * cus;
+  const double by_d = a->D == 128 ? 1.0 : 0.7;
+  const double load = 0.85 * (double)wgs * (double)units / (3 * cus);
+  const double items = shared ? 14 + by_d * load : 8 + by_d * std::max(0.19 * (double)units, load);
+  const int64_t parts = (int64_t)p.tiles * a->HKV * p.nsplit, rounds = (parts + 2 * cus - 1) / (2 * cus);
+  const double tiles = (p.nsplit > 1 ? 20 : 10) +
+                       by_d * (parts <= cus ? 1.35 : 2.4 * (double)rounds) * (double)((p.chunks + p.nsplit - 1) / p.nsplit);
+  return items <= 1.1 * tiles;
 }
 
 template <typename T, int KV, int D, bool ONE>
@@ -607,7 +627,8 @@ using namespace srswa;
 
 extern "C" size_t srswa_cache8_prefill_workspace(const srswa_cache8_attend_args* a) {
   if (!cache8_plannable(a)) return 0;
-  return narrow(a) ? cache8_decode_ws(a) : ws_bytes_of(plan(a));
+  const PrefillK p = plan(a);
+  return narrow(a, p) ? cache8_decode_ws(a) : ws_bytes_of(p);
 }
 
 extern "C" int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -623,8 +644,8 @@ extern "C" int srswa_cache8_prefill(const srswa_cache8_attend_args* a, void* ws,
     set_error("%s: cu_seqlens_q is null", what);
     return SRSWA_INVALID;
   }
-  if (narrow(a)) return cache8_decode_run(a, ws, ws_bytes, stream, what);
   PrefillK p = plan(a);
+  if (narrow(a, p)) return cache8_decode_run(a, ws, ws_bytes, stream, what);
   const size_t need = ws_bytes_of(p);
   if (need > 0 && (!ws || ws_bytes < need)) {
     set_error("%s: workspace of %zu bytes required (got %zu)", what, need, ws_bytes);
