@@ -47,7 +47,8 @@ constexpr int kMinShare = 16;
 struct AttendK {
   srswa_cache8_attend_args a;
   int G;                  // query heads per kv head
-  int tiles, items;       // row tiles per request, items in all (R * tiles)
+  int tiles, items;       // row tiles per request at most, items in all
+  bool dense;             // items numbered by the rows there are (tile_at), else R * tiles
   int shares;             // workgroups per kv head that share the items' units; 0: one per item
   bool pairs;             // D = 64: neighbouring heads to one XCD
   int rs;                 // rows of a record
@@ -105,11 +106,30 @@ __device__ __forceinline__ Tile tile_of(const AttendK& p, int r, int tile) {
   return t;
 }
 
+// Item number `item`.  Where the requests' lengths are far below their bound, the items
+// are numbered by the rows there are: request r's from first(r) = 16-row tiles before
+// its first row + r on, which leaves every request as many as its rows can take.
+template <bool SEL>
+__device__ __forceinline__ Tile tile_at(const AttendK& p, int item) {
+  if (!p.dense) return tile_of<SEL>(p, item / p.tiles, item % p.tiles);
+  const srswa_cache8_attend_args& a = p.a;
+  auto first = [&](int r) {
+    return (int)((int64_t)min(max(a.cu_seqlens_q[r], 0), a.total_q) * p.G / kRows) + r;
+  };
+  int lo = 0, hi = a.R - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (first(mid) <= item) lo = mid;
+    else hi = mid - 1;
+  }
+  return tile_of<SEL>(p, lo, max(item - first(lo), 0));
+}
+
 // Units that an item counts for: one at least, so that a row without keys is written.
 template <bool SEL>
 __device__ __forceinline__ uint32_t item_units(const AttendK& p, int item) {
   if (item >= p.items) return 0u;
-  const Tile t = tile_of<SEL>(p, item / p.tiles, item % p.tiles);
+  const Tile t = tile_at<SEL>(p, item);
   return t.nrows > 0 ? (uint32_t)max(t.units, 1) : 0u;
 }
 
@@ -546,7 +566,7 @@ __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
     id = (int)blockIdx.x / a.HKV;
   }
   if (p.shares == 0) {
-    const Tile t = tile_of<SEL>(p, id / p.tiles, id % p.tiles);
+    const Tile t = tile_at<SEL>(p, id);
     if (t.nrows > 0) attend_item<T, KV, D, SEL, MIX, NW>(p, h, t, 0, t.units, nullptr);
     return;
   }
@@ -557,7 +577,7 @@ __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
   int item = sh.item;
   float* recs = p.part + ((int64_t)id * a.HKV + h) * 2 * p.rs * (D + 2);
   for (bool first = true; s < e; ++item) {
-    const Tile t = tile_of<SEL>(p, item / p.tiles, item % p.tiles);
+    const Tile t = tile_at<SEL>(p, item);
     if (t.nrows == 0) continue;
     const int64_t end = start + max(t.units, 1);
     const bool whole = s == start && e >= end;
@@ -580,7 +600,7 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void cache8_merge_kernel(Atten
   const srswa_cache8_attend_args& a = p.a;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int rr = (int)blockIdx.x % p.rs, h = (int)blockIdx.x / p.rs % a.HKV, item = (int)blockIdx.x / p.rs / a.HKV;
-  const Tile t = tile_of<SEL>(p, item / p.tiles, item % p.tiles);
+  const Tile t = tile_at<SEL>(p, item);
   if (rr >= t.nrows) return;
   int64_t start = 0, total = 0;
   for (int i0 = 0; i0 < p.items; i0 += kWave) {
@@ -717,7 +737,9 @@ AttendK plan(const srswa_cache8_attend_args* a) {
   p.scale_l2 = a->scale * kLog2e;
   const int64_t rows = (int64_t)a->max_query_len * p.G;
   p.tiles = (int)(a->topk ? (int64_t)a->max_query_len * ((p.G + kRows - 1) / kRows) : (rows + kRows - 1) / kRows);
-  const int64_t items = (int64_t)a->R * p.tiles;
+  const int64_t even = (int64_t)a->R * p.tiles, own = (int64_t)a->total_q * p.G / kRows + a->R;
+  p.dense = a->cu_seqlens_q && own < even;
+  const int64_t items = p.dense ? own : even;
   p.items = (int)std::min<int64_t>(items, INT32_MAX);
   p.rs = (int)std::min<int64_t>(kRows, a->topk ? p.G : rows);
   int64_t groups = (int64_t)a->max_blocks * a->page_size / kGroup;
@@ -776,7 +798,7 @@ int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_byt
   p.part = reinterpret_cast<float*>(ws);
   const int64_t wgs = (int64_t)(p.shares > 0 ? p.shares : p.items) * a->HKV;
   const int64_t grid = p.pairs ? (wgs / 2 + 7) / 8 * 16 : wgs;
-  if (grid > 0x7fffffff || (int64_t)a->R * p.tiles * a->HKV * p.rs > 0x7fffffff) {
+  if (grid > 0x7fffffff || (int64_t)p.items * a->HKV * p.rs > 0x7fffffff) {
     set_error("%s: grid too large", what);
     return SRSWA_UNSUPPORTED;
   }
@@ -790,7 +812,7 @@ size_t cache8_decode_ws(const srswa_cache8_attend_args* a) { return ws_bytes_of(
 
 void cache8_decode_load(const srswa_cache8_attend_args* a, int64_t* wgs, int64_t* units, bool* shared) {
   const AttendK p = plan(a);
-  *wgs = std::min<int64_t>((int64_t)a->R * p.tiles, (int64_t)a->total_q * p.G / kRows + a->R) * a->HKV;
+  *wgs = (int64_t)p.items * a->HKV;
   *units = p.most_units;
   *shared = p.shares > 0;
 }
