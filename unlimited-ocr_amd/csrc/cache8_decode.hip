@@ -51,7 +51,7 @@ struct AttendK {
   bool dense;             // items numbered by the rows there are (tile_at), else R * tiles
   int shares;             // workgroups per kv head that share the items' units; 0: one per item
   bool pairs;             // D = 64: neighbouring heads to one XCD
-  int rs;                 // rows of a record
+  int rs, rm;             // rows of a record, rows that a workgroup of the merge joins
   int gpp;                // 16-key groups per page
   int64_t most_units;     // of an item
   float scale_l2;         // scale * log2(e)
@@ -589,19 +589,24 @@ __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
   }
 }
 
-// Joins the shares of an item that was cut: one workgroup per (item, kv head, row), a
-// wave for each eighth record, D / 64 dims a lane.  Share i begins with the item (its
-// first record) unless the item starts inside it (its last).  One request of 30,000
-// keys, 59 records a row: 42.9 us with one wave, 29.8 with four, 28.8 with eight.
+// Joins the shares of an item that was cut: one workgroup per (item, kv head, rm rows),
+// D / 64 dims a lane, its eight waves shared among the rows, or a row's records among
+// waves where rows are few (one request of 30,000 keys, 59 records a row: 42.9 us with
+// one wave, 29.8 with four, 28.8 with eight).  rm is as small as 2,048 workgroups allow
+// (16 rows after 30,000 keys: 32 us with a row each, 73 with all 16; 256 requests of 4
+// rows 460 and 392).  Share i begins with the item (its first
+// record) unless the item starts inside it (its last).
 template <typename T, int D, bool SEL>
 __global__ __launch_bounds__(kMergeWaves * kWave) void cache8_merge_kernel(AttendK p) {
   constexpr int DL = D / kWave;
   __shared__ float s_o[kMergeWaves][D], s_l[kMergeWaves];
   const srswa_cache8_attend_args& a = p.a;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int rr = (int)blockIdx.x % p.rs, h = (int)blockIdx.x / p.rs % a.HKV, item = (int)blockIdx.x / p.rs / a.HKV;
+  const int parts = (p.rs + p.rm - 1) / p.rm, id = (int)blockIdx.x / parts;
+  const int h = id % a.HKV, item = id / a.HKV;
   const Tile t = tile_at<SEL>(p, item);
-  if (rr >= t.nrows) return;
+  const int first = (int)blockIdx.x % parts * p.rm, last = min(first + p.rm, t.nrows);
+  if (first >= last) return;
   int64_t start = 0, total = 0;
   for (int i0 = 0; i0 < p.items; i0 += kWave) {
     const int n = (int)item_units<SEL>(p, i0 + lane);
@@ -620,43 +625,53 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void cache8_merge_kernel(Atten
   const int s0 = share_of(start), s1 = share_of(end - 1);
   if (s0 == s1) return;                          // not cut
   const int64_t rsz = (int64_t)p.rs * (D + 2);
-  auto record = [&](int i) {
-    return p.part + (((int64_t)i * a.HKV + h) * 2 + (i == s0 && total * i / n != start ? 1 : 0)) * rsz;
-  };
-  float M = -INFINITY;
-  for (int i = s0 + lane; i <= s1; i += kWave) M = fmaxf(M, record(i)[p.rs * D + rr]);
-  M = wave_max(M);
-  float o[DL] = {}, L = 0.f;
+  const int late = total * s0 / n != start ? 1 : 0;
+  auto record = [&](int i) { return p.part + (((int64_t)i * a.HKV + h) * 2 + (i == s0 ? late : 0)) * rsz; };
+  int per = kMergeWaves;                         // waves per row
+  while (per > 1 && per * (last - first) > kMergeWaves) per >>= 1;
+  const int sub = wave % per;
+  for (int r0 = first; r0 < last; r0 += kMergeWaves / per) {
+    const int rr = r0 + wave / per;
+    float M = -INFINITY, o[DL] = {}, L = 0.f;
+    if (rr < last) {
+      for (int i = s0 + lane; i <= s1; i += kWave) M = fmaxf(M, record(i)[p.rs * D + rr]);
+      M = wave_max(M);
 #pragma unroll 8
-  for (int i = s0 + wave; i <= s1; i += kMergeWaves) {
-    const float* rec = record(i);
-    const float mk = rec[p.rs * D + rr];
-    const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
-    L = fmaf(f, rec[p.rs * D + p.rs + rr], L);
+      for (int i = s0 + sub; i <= s1; i += per) {
+        const float* rec = record(i);
+        const float mk = rec[p.rs * D + rr];
+        const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
+        L = fmaf(f, rec[p.rs * D + p.rs + rr], L);
 #pragma unroll
-    for (int d = 0; d < DL; ++d) o[d] = fmaf(f, rec[rr * D + DL * lane + d], o[d]);
+        for (int d = 0; d < DL; ++d) o[d] = fmaf(f, rec[rr * D + DL * lane + d], o[d]);
+      }
+    }
+    if (per > 1) {
+      if (r0 > first) __syncthreads();           // the rows before are read
+#pragma unroll
+      for (int d = 0; d < DL; ++d) s_o[wave][DL * lane + d] = o[d];
+      if (lane == 0) s_l[wave] = L;
+      __syncthreads();
+#pragma unroll
+      for (int w = 1; w < kMergeWaves; ++w) {
+        const int from = min(wave + w, kMergeWaves - 1);
+        L += w < per ? s_l[from] : 0.f;
+#pragma unroll
+        for (int d = 0; d < DL; ++d) o[d] += w < per ? s_o[from][DL * lane + d] : 0.f;
+      }
+    }
+    if (sub > 0 || rr >= last) continue;
+    const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
+    const float inv = inv_sum(M, L);
+    T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn + (int64_t)ho * a.o_sh + DL * lane;
+    if constexpr (DL == 2) {
+      *reinterpret_cast<uint32_t*>(op) = Mfma<T>::pack2(o[0] * inv, o[1] * inv);
+    } else {
+      *reinterpret_cast<uint16_t*>(op) = (uint16_t)(Mfma<T>::pack2(o[0] * inv, 0.f) & 0xffffu);
+    }
+    if (a.lse && lane == 0)
+      a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] = lse_of(M, L);
   }
-#pragma unroll
-  for (int d = 0; d < DL; ++d) s_o[wave][DL * lane + d] = o[d];
-  if (lane == 0) s_l[wave] = L;
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int w = 1; w < kMergeWaves; ++w) {
-    L += s_l[w];
-#pragma unroll
-    for (int d = 0; d < DL; ++d) o[d] += s_o[w][DL * lane + d];
-  }
-  const int ro = t.row0 + rr, ho = h * p.G + ro % p.G;
-  const float inv = inv_sum(M, L);
-  T* op = reinterpret_cast<T*>(a.out) + (int64_t)(t.q0 + ro / p.G) * a.o_sn + (int64_t)ho * a.o_sh + DL * lane;
-  if constexpr (DL == 2) {
-    *reinterpret_cast<uint32_t*>(op) = Mfma<T>::pack2(o[0] * inv, o[1] * inv);
-  } else {
-    *reinterpret_cast<uint16_t*>(op) = (uint16_t)(Mfma<T>::pack2(o[0] * inv, 0.f) & 0xffffu);
-  }
-  if (a.lse && lane == 0)
-    a.lse[(int64_t)(t.q0 + ro / p.G) * a.lse_sn + (int64_t)ho * a.lse_sh] = lse_of(M, L);
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -742,6 +757,8 @@ AttendK plan(const srswa_cache8_attend_args* a) {
   const int64_t items = p.dense ? own : even;
   p.items = (int)std::min<int64_t>(items, INT32_MAX);
   p.rs = (int)std::min<int64_t>(kRows, a->topk ? p.G : rows);
+  p.rm = 1;
+  while (p.rm < p.rs && items * a->HKV * ((p.rs + p.rm - 1) / p.rm) > 2048) p.rm *= 2;
   int64_t groups = (int64_t)a->max_blocks * a->page_size / kGroup;
   if (a->topk) groups = (int64_t)a->topk_n * p.gpp + std::min<int64_t>(groups, a->window / kGroup + 2);
   else if (a->window > 0)
@@ -768,7 +785,7 @@ void launch(const AttendK& p, unsigned grid, hipStream_t st) {
   if (kMix && p.a.max_query_len > 1) cache8_decode_kernel<T, KV, D, SEL, kMix, 4><<<grid, 4 * kWave, 0, st>>>(p);
   else cache8_decode_kernel<T, KV, D, SEL, false, 4><<<grid, 4 * kWave, 0, st>>>(p);
   if (p.shares > 0)
-    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.items * p.a.HKV * p.rs), kMergeWaves * kWave, 0, st>>>(p);
+    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.items * p.a.HKV * ((p.rs + p.rm - 1) / p.rm)), kMergeWaves * kWave, 0, st>>>(p);
 }
 template <typename T, int KV, int D>
 void launch_sel(const AttendK& p, unsigned grid, hipStream_t st) {
@@ -798,7 +815,7 @@ int cache8_decode_run(const srswa_cache8_attend_args* a, void* ws, size_t ws_byt
   p.part = reinterpret_cast<float*>(ws);
   const int64_t wgs = (int64_t)(p.shares > 0 ? p.shares : p.items) * a->HKV;
   const int64_t grid = p.pairs ? (wgs / 2 + 7) / 8 * 16 : wgs;
-  if (grid > 0x7fffffff || (int64_t)p.items * a->HKV * p.rs > 0x7fffffff) {
+  if (grid > 0x7fffffff || (int64_t)p.items * a->HKV * ((p.rs + p.rm - 1) / p.rm) > 0x7fffffff) {
     set_error("%s: grid too large", what);
     return SRSWA_UNSUPPORTED;
   }
