@@ -769,7 +769,8 @@ AttendK plan(const srswa_cache8_attend_args* a) {
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
   if (units > 128 || (units > 64 && wgs <= 64))
-    p.shares = (int)std::min<int64_t>(std::max(1, (a->D == 64 ? 4 : 3) * cus / a->HKV), (units * p.items + kMinShare - 1) / kMinShare);
+    p.shares = (int)std::min<int64_t>(std::max(1, (a->D == 64 ? 4 : 3) * cus / a->HKV),
+                                      (units * p.items + kMinShare - 1) / kMinShare);
   return p;
 }
 
@@ -785,7 +786,8 @@ void launch(const AttendK& p, unsigned grid, hipStream_t st) {
   if (kMix && p.a.max_query_len > 1) cache8_decode_kernel<T, KV, D, SEL, kMix, 4><<<grid, 4 * kWave, 0, st>>>(p);
   else cache8_decode_kernel<T, KV, D, SEL, false, 4><<<grid, 4 * kWave, 0, st>>>(p);
   if (p.shares > 0)
-    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.items * p.a.HKV * ((p.rs + p.rm - 1) / p.rm)), kMergeWaves * kWave, 0, st>>>(p);
+    cache8_merge_kernel<T, D, SEL><<<(unsigned)(p.items * p.a.HKV * ((p.rs + p.rm - 1) / p.rm)),
+                                     kMergeWaves * kWave, 0, st>>>(p);
 }
 template <typename T, int KV, int D>
 void launch_sel(const AttendK& p, unsigned grid, hipStream_t st) {
